@@ -2,6 +2,7 @@
 // dtypes and contiguity, allocates outputs with the caching allocator and launches on the
 // current CUDA stream. Launch errors raise immediately.
 #include <torch/extension.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
@@ -1005,6 +1006,112 @@ void seen_mark(at::Tensor seen, at::Tensor ids, int64_t vocab) {
         "seen_mark");
 }
 
+// ---------------------------------------------------------------- 8-bit MLA latent cache
+kimi::MlaCacheInts cache_ints(const at::Tensor& t, int64_t batch, const at::Device& dev, const char* name) {
+  TORCH_CHECK(t.device() == dev && t.dim() == 1 && t.size(0) == batch &&
+                  (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong) &&
+                  (batch <= 1 || t.stride(0) == 1),
+              name, " must be a contiguous int32 or int64 [B] tensor on the cache's device");
+  kimi::MlaCacheInts v;
+  v.p = t.data_ptr();
+  v.is64 = t.scalar_type() == at::kLong;
+  return v;
+}
+
+kimi::MlaCacheView cache_view(const at::Tensor& codes, const at::Tensor& scales) {
+  TORCH_CHECK(codes.is_cuda() && codes.dim() == 3 && codes.scalar_type() == at::kFloat8_e4m3fn,
+              "codes must be a CUDA float8_e4m3fn [B, slots, L] tensor");
+  TORCH_CHECK(codes.size(2) > 0 && (codes.size(2) == 1 || codes.stride(2) == 1),
+              "codes must be contiguous along the latent axis");
+  TORCH_CHECK(scales.device() == codes.device() && scales.dim() == 2 && scales.scalar_type() == at::kFloat &&
+                  scales.size(0) == codes.size(0) && scales.size(1) == codes.size(1),
+              "scales must be a float32 [B, slots] tensor on the codes' device");
+  TORCH_CHECK(codes.size(0) <= 65535 && codes.size(2) <= (1 << 20), "cache batch or latent width too large");
+  kimi::MlaCacheView v;
+  v.codes = static_cast<uint8_t*>(codes.data_ptr());
+  v.scales = scales.data_ptr<float>();
+  v.code_b = codes.stride(0);
+  v.code_t = codes.stride(1);
+  v.scale_b = scales.stride(0);
+  v.scale_t = scales.stride(1);
+  v.slots = codes.size(1);
+  v.width = (int)codes.size(2);
+  return v;
+}
+
+void mla_cache_write(at::Tensor latent, at::Tensor codes, at::Tensor scales, at::Tensor offsets,
+                     c10::optional<at::Tensor> counts) {
+  kimi::MlaCacheWriteArgs a;
+  a.cache = cache_view(codes, scales);
+  at::assert_no_internal_overlap(codes);
+  at::assert_no_internal_overlap(scales);
+  TORCH_CHECK(latent.device() == codes.device() && latent.dim() == 3 && latent.size(0) == codes.size(0) &&
+                  latent.size(2) == codes.size(2),
+              "latent must be a [B, T, L] tensor with the codes' device, batch and latent width");
+  const int dt = dtype_code(latent);
+  const at::cuda::CUDAGuard gd(codes.device());
+  if (latent.size(2) > 1 && latent.stride(2) != 1) latent = latent.contiguous();
+  a.x = latent.data_ptr();
+  a.x_b = latent.stride(0);
+  a.x_t = latent.stride(1);
+  a.batch = (int)latent.size(0);
+  a.tokens = latent.size(1);
+  a.offsets = cache_ints(offsets, a.batch, codes.device(), "offsets");
+  if (counts.has_value() && counts->defined()) a.counts = cache_ints(*counts, a.batch, codes.device(), "counts");
+  check(kimi::mla_cache_write(dt, a, stream()), "mla_cache_write");
+}
+
+at::Tensor mla_cache_read(at::Tensor codes, at::Tensor scales, c10::optional<at::Tensor> lengths, at::ScalarType dtype,
+                          int64_t tokens) {
+  kimi::MlaCacheReadArgs a;
+  a.cache = cache_view(codes, scales);
+  TORCH_CHECK(tokens >= 0 && tokens <= a.cache.slots, "tokens must lie in [0, slots]");
+  const at::cuda::CUDAGuard gd(codes.device());
+  auto out = at::empty({codes.size(0), tokens, codes.size(2)}, codes.options().dtype(dtype));
+  a.out = out.data_ptr();
+  a.batch = (int)codes.size(0);
+  a.tokens = tokens;
+  if (lengths.has_value() && lengths->defined()) a.lengths = cache_ints(*lengths, a.batch, codes.device(), "lengths");
+  check(kimi::mla_cache_read(dtype_code(out), a, stream()), "mla_cache_read");
+  return out;
+}
+
+at::Tensor mla_cache_attention(at::Tensor q, at::Tensor codes, at::Tensor scales, at::Tensor lengths,
+                               c10::optional<at::Tensor> start, double scale) {
+  kimi::MlaCacheAttnArgs a;
+  a.cache = cache_view(codes, scales);
+  TORCH_CHECK(q.device() == codes.device() && q.dim() == 4 && q.size(0) == codes.size(0) && q.size(3) == codes.size(2),
+              "query_latent must be a [B, Tq, H, L] tensor with the codes' device, batch and latent width");
+  TORCH_CHECK(kimi::mla_cache_attn_supported(a.cache.width), "latent widths up to 2048 are supported, got " +
+                                                                   std::to_string(a.cache.width));
+  const int dt = dtype_code(q);
+  TORCH_CHECK(q.size(1) * q.size(2) <= (1 << 19), "too many query rows per sequence");
+  const at::cuda::CUDAGuard gd(codes.device());
+  if (q.size(3) > 1 && q.stride(3) != 1) q = q.contiguous();
+  a.q = q.data_ptr();
+  a.q_b = q.stride(0);
+  a.q_i = q.stride(1);
+  a.q_h = q.stride(2);
+  a.batch = (int)q.size(0);
+  a.queries = (int)q.size(1);
+  a.heads = (int)q.size(2);
+  a.scale = (float)scale;
+  a.lengths = cache_ints(lengths, a.batch, codes.device(), "lengths");
+  if (start.has_value() && start->defined()) a.start = cache_ints(*start, a.batch, codes.device(), "query_start");
+  auto out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+  if (out.numel() == 0) return out;
+  if (a.cache.slots == 0) return out.zero_();
+  a.out = out.data_ptr();
+  const int64_t floats = kimi::mla_cache_attn_workspace(dt, a);
+  at::Tensor work;
+  if (floats) {
+    work = at::empty({floats}, q.options().dtype(at::kFloat));
+    a.part_acc = work.data_ptr<float>();
+  }
+  check(kimi::mla_cache_attn(dt, a, stream()), "mla_cache_attention");
+  return out;
+}
+
 // ---------------------------------------------------------------- expert-parallel comm
 // `ptrs`: nine regions x world peer addresses, region-major (flags, counts, xs, row_token,
 // row_weight, agg, dagg, dxs, dw_row).
@@ -1231,6 +1338,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kda_decode", &kda_decode);
   m.def("mla_decode_supported", &mla_decode_supported);
   m.def("mla_decode", &mla_decode);
+  m.def("mla_cache_write", &mla_cache_write);
+  m.def("mla_cache_read", &mla_cache_read);
+  m.def("mla_cache_attention", &mla_cache_attention);
   m.def("sample_tokens", &sample_tokens);
   m.def("seen_mark", &seen_mark);
   m.def("rms_norm_bwd", &rms_norm_bwd);

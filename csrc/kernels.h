@@ -152,6 +152,50 @@ cudaError_t sample_tokens(int dtype, const void* logits, int batch, int vocab, c
 cudaError_t seen_mark(uint32_t* seen, int seen_words, const int64_t* ids, int64_t rows, int64_t cols, int64_t ld,
                       int vocab, cudaStream_t s);
 
+// ---------------------------------------------------------------- 8-bit MLA latent cache
+// Format and device helpers: mla_cache.cuh.  Strides are in elements; the latent axis is contiguous.
+struct MlaCacheInts {  // [B] int32 or int64 as the caller keeps them; p == nullptr: not given
+  const void* p = nullptr;
+  int is64 = 0;
+};
+struct MlaCacheView {
+  uint8_t* codes = nullptr;  // [B, slots, width] e4m3
+  float* scales = nullptr;   // [B, slots]
+  int64_t code_b = 0, code_t = 0, scale_b = 0, scale_t = 0;
+  int64_t slots = 0;
+  int width = 0;
+};
+struct MlaCacheWriteArgs {
+  MlaCacheView cache;
+  const void* x = nullptr;  // [batch, tokens, width]
+  int64_t x_b = 0, x_t = 0;
+  MlaCacheInts offsets, counts;
+  int batch = 0;
+  int64_t tokens = 0;
+};
+struct MlaCacheReadArgs {
+  MlaCacheView cache;
+  void* out = nullptr;  // [batch, tokens, width] contiguous
+  MlaCacheInts lengths;
+  int batch = 0;
+  int64_t tokens = 0;
+};
+struct MlaCacheAttnArgs {
+  MlaCacheView cache;
+  const void* q = nullptr;  // [batch, queries, heads, width]
+  int64_t q_b = 0, q_i = 0, q_h = 0;
+  MlaCacheInts lengths, start;
+  int batch = 0, queries = 0, heads = 0;
+  float scale = 1.f;
+  void* out = nullptr;       // [batch, queries, heads, width] contiguous
+  float* part_acc = nullptr;  // mla_cache_attn_workspace() floats: partial contexts, then (max, sum) pairs
+};
+cudaError_t mla_cache_write(int dtype, const MlaCacheWriteArgs& a, cudaStream_t s);
+cudaError_t mla_cache_read(int dtype, const MlaCacheReadArgs& a, cudaStream_t s);
+bool mla_cache_attn_supported(int width);
+int64_t mla_cache_attn_workspace(int dtype, const MlaCacheAttnArgs& a);
+cudaError_t mla_cache_attn(int dtype, const MlaCacheAttnArgs& a, cudaStream_t s);
+
 // ---------------------------------------------------------------- expert-parallel comm (ep_comm.cu)
 // Pointers into every rank's symmetric buffer (index = rank in the expert group).
 struct EpPeers {

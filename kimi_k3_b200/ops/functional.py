@@ -485,6 +485,45 @@ def mla_absorbed_decode(query, latent_cache, cache_mask, key_up_weight, value_up
     return out[:, None]
 
 
+# --------------------------------------------------------------------------- 8-bit MLA latent cache
+def _serving_only(x: torch.Tensor, name: str) -> None:
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{name} has no backward: the 8-bit latent cache is a serving structure "
+                           "(call it under torch.no_grad() or torch.inference_mode())")
+
+
+def mla_cache_write(latent, codes, scales, offsets, counts=None) -> None:
+    """Quantise latents into an 8-bit MLA cache, in place.
+
+    ``latent`` ``[B,T,L]`` (fp32 / bf16 / fp16, any batch and token strides); ``codes`` ``[B,slots,L]``
+    float8_e4m3fn and ``scales`` ``[B,slots]`` fp32 with value = code * scale.  Token j of sequence b
+    goes to slot ``offsets[b] + j`` for ``j < counts[b]`` (all T without ``counts``); slots outside the
+    buffer are dropped.  A token's scale is the least power of two 2^k, k >= -126, under which its
+    largest magnitude fits e4m3 (448 * 2^k); a token holding a NaN or an infinity gets scale NaN and
+    codes 0.  ``offsets`` and ``counts`` are int32 or int64 ``[B]`` device tensors."""
+    _serving_only(latent, "mla_cache_write")
+    _C().mla_cache_write(latent, codes, scales, offsets, counts)
+
+
+def mla_cache_read(codes, scales, lengths=None, *, dtype=torch.bfloat16, tokens: int | None = None) -> torch.Tensor:
+    """Values of the first ``tokens`` slots (default: all) of an 8-bit MLA cache -> ``[B,tokens,L]`` in
+    ``dtype``; slots at or past ``lengths[b]`` read as zeros.  Exact in bf16 and fp32 (a code has four
+    significant bits and the scale is a power of two)."""
+    return _C().mla_cache_read(codes, scales, lengths, dtype, codes.shape[1] if tokens is None else int(tokens))
+
+
+def mla_cache_attention(query_latent, codes, scales, lengths, *, query_start=None, scale: float = 1.0) -> torch.Tensor:
+    """Attention of ``query_latent`` ``[B,Tq,H,L]`` (queries absorbed into the latent space, any strides
+    outside the last axis) over an 8-bit MLA cache -> contexts ``[B,Tq,H,L]`` in the query's type.
+
+    The cached latent is key and value of every head.  Query token i of sequence b stands at position
+    ``query_start[b] + i`` (default ``lengths[b] - Tq + i``: the last Tq cached tokens) and sees the slots
+    below ``lengths[b]`` up to its own position; a query that sees none gets zeros.  Scores are
+    multiplied by ``scale``.  Softmax statistics and contexts are held in fp32."""
+    _serving_only(query_latent, "mla_cache_attention")
+    return _C().mla_cache_attention(query_latent, codes, scales, lengths, query_start, float(scale))
+
+
 # --------------------------------------------------------------------------- sampling
 def sample_tokens(logits, seen_bits, config, seed_offset):
     """Fused next-token choice for ``[B,V]`` logits -> ``[B]`` int64 (one launch).
