@@ -1341,6 +1341,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("mla_cache_write", &mla_cache_write);
   m.def("mla_cache_read", &mla_cache_read);
   m.def("mla_cache_attention", &mla_cache_attention);
+  m.def("mla_cache_status", [](bool clear) {
+    const int v = kimi::mla_cache_status(clear);
+    TORCH_CHECK(v >= 0, "reading the MLA cache status word failed");
+    return v;
+  });
   m.def("sample_tokens", &sample_tokens);
   m.def("seen_mark", &seen_mark);
   m.def("rms_norm_bwd", &rms_norm_bwd);

@@ -195,6 +195,9 @@ cudaError_t mla_cache_read(int dtype, const MlaCacheReadArgs& a, cudaStream_t s)
 bool mla_cache_attn_supported(int width);
 int64_t mla_cache_attn_workspace(int dtype, const MlaCacheAttnArgs& a);
 cudaError_t mla_cache_attn(int dtype, const MlaCacheAttnArgs& a, cudaStream_t s);
+// Device status word of the attention's bounded waits (0 = ok), read and cleared by the host.
+int mla_cache_status(bool clear);
+int* mla_cache_default_status();
 
 // ---------------------------------------------------------------- expert-parallel comm (ep_comm.cu)
 // Pointers into every rank's symmetric buffer (index = rank in the expert group).

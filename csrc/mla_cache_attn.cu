@@ -11,6 +11,7 @@
 // unnormalised context, and a second kernel joins the splits.
 #include "device_info.h"
 #include "mla_cache.cuh"
+#include "mla_cache_attn.h"
 
 namespace kimi {
 namespace {
@@ -266,7 +267,7 @@ cudaError_t launch_any(const MlaCacheAttnArgs& a, cudaStream_t s) {
 bool mla_cache_attn_supported(int width) { return width > 0 && width <= 2048; }
 
 int64_t mla_cache_attn_workspace(int dtype, const MlaCacheAttnArgs& a) {
-  (void)dtype;
+  if (mla_attn_tc_supported(dtype, a)) return mla_attn_tc_workspace(dtype, a);
   const int splits = generic_splits(a);
   return splits == 1 ? 0 : (int64_t)a.batch * splits * a.queries * a.heads * (a.cache.width + 2);
 }
@@ -274,6 +275,7 @@ int64_t mla_cache_attn_workspace(int dtype, const MlaCacheAttnArgs& a) {
 cudaError_t mla_cache_attn(int dtype, const MlaCacheAttnArgs& a, cudaStream_t s) {
   if (a.batch <= 0 || a.queries <= 0 || a.heads <= 0) return cudaSuccess;
   if (!mla_cache_attn_supported(a.cache.width)) return cudaErrorInvalidValue;
+  if (mla_attn_tc_supported(dtype, a)) return mla_attn_tc(dtype, a, s);
   switch (dtype) {
     case 0: return launch_any<float>(a, s);
     case 1: return launch_any<__nv_bfloat16>(a, s);
