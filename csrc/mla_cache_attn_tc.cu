@@ -54,6 +54,7 @@ constexpr int kBox = kTile * 128;          // bytes of a box
 constexpr int kThreads = 320;
 constexpr int kMaxSlots = 32;              // ring slots
 constexpr int kSmemMax = 227 * 1024;
+constexpr int kOcts = 8;                   // 8-element pieces of a query row per lane: widths up to 2,048
 constexpr float kTop = 15.f;               // a weight may reach 2^kTop
 constexpr float kRoom = 4.f;               // a new reference leaves this many bits
 constexpr float kSumRoom = 40.f;           // the sums' reference may lag by this many bits
@@ -65,6 +66,10 @@ struct Plan {
   int boxes = 0;       // boxes of a tile: ceil(L / 128)
   int slots = 0;       // ring slots
   int s_bufs = 0;
+  int stack = 0;       // weight parts side by side on N
+  int runs = 0;        // context products of a box: ceil(parts / stack)
+  int np = 0;          // N of the context product
+  int p_bytes = 0;     // one weight buffer
   int ahead = 0;       // boxes of the next tile's scores issued before this tile's context product
   uint32_t tmem = 0;
   size_t smem = 0;
@@ -75,7 +80,8 @@ struct Plan {
 struct TcParams {
   CUtensorMap map;
   MlaCacheAttnArgs a;
-  int rows, rows_tile, row_tiles, boxes, slots, s_bufs, ahead, direct, min_tiles, t_first;
+  int rows, rows_tile, row_tiles, boxes, slots, s_bufs, ahead, direct, min_tiles, t_first, q_vec;
+  int stack, runs, np, p_bytes;
   uint32_t tmem;
   int64_t z_mul;       // 0 when every sequence reads the same cache rows
   float* part_o;       // [grid + pairs][rows_tile][L]
@@ -88,13 +94,16 @@ constexpr int pad16(int n) { return (n + 15) / 16 * 16; }
 // QP parts of a query row; QP + 1 parts of a weight.
 template <int RH, int QP>
 struct Shape {
+  static constexpr int R = 2 * RH;          // rows, padded
+  static constexpr int NS = pad16(QP * R);  // N of the score product
   static constexpr int WP = QP + 1;
-  static constexpr int R = 2 * RH;             // rows, padded
-  static constexpr int NS = pad16(QP * R);     // N of the score product
-  static constexpr int NP = pad16(R);          // N of the context product
-  static constexpr int P_BYTES = NP * 128 * ((WP + 1) / 2);  // one weight buffer
 };
 
+KIMI_D bool elect_one() {
+  uint32_t e;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(e));
+  return e != 0;
+}
 KIMI_D void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
@@ -103,7 +112,7 @@ KIMI_D void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t 
       : "memory");
 }
 // kind::f8f6f4 instruction descriptor: fp32 accumulator, A e4m3 (0), B e4m3 (0) or e5m2 (1).
-constexpr uint32_t idesc_f8(int m, int n, bool a_mn, bool b_e5m2) {
+__host__ __device__ constexpr uint32_t idesc_f8(int m, int n, bool a_mn, bool b_e5m2) {
   return (1u << 4) | ((b_e5m2 ? 1u : 0u) << 10) | ((a_mn ? 1u : 0u) << 15) | ((uint32_t)(n >> 3) << 17) |
          ((uint32_t)(m >> 4) << 24);
 }
@@ -114,6 +123,29 @@ KIMI_D void tmem_ld4(uint32_t addr, float* v) {
                : "r"(addr));
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(r[i]);
+}
+// N columns of lanes 0-15 for each half of the warp: threads 16-31 get the columns SPLIT further on.
+template <int N, int SPLIT>
+KIMI_D void tmem_ld_halves(uint32_t addr, float* v) {
+  if constexpr (N == 2) {
+    uint32_t r[2];
+    asm volatile("tcgen05.ld.sync.aligned.16x32bx2.x2.b32 {%0,%1}, [%2], %3;\n"
+                 : "=r"(r[0]), "=r"(r[1])
+                 : "r"(addr), "n"(SPLIT));
+    v[0] = __uint_as_float(r[0]);
+    v[1] = __uint_as_float(r[1]);
+  } else if constexpr (N == 4) {
+    uint32_t r[4];
+    asm volatile("tcgen05.ld.sync.aligned.16x32bx2.x4.b32 {%0,%1,%2,%3}, [%4], %5;\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr), "n"(SPLIT));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(r[i]);
+  } else {
+    constexpr int H = N % 4 ? N - 2 : N - 4;
+    tmem_ld_halves<H, SPLIT>(addr, v);
+    tmem_ld_halves<N - H, SPLIT>(addr + H, v + H);
+  }
 }
 KIMI_D float tmem_ld1(uint32_t addr) {
   uint32_t r;
@@ -136,10 +168,26 @@ KIMI_D bool group_any(int id, bool v) {
   return r != 0;
 }
 KIMI_D float pow2i(int k) { return __uint_as_float((uint32_t)(k + 127) << 23); }
-// v * 2^e for any integer-valued e, exact while the result is a normal number.
-KIMI_D float scale2(float v, float e) {
+// 2^e as two factors, for any integer-valued e: their product is applied one at a time.
+KIMI_D float2 pow2_pair(float e) {
   const int n = (int)fminf(fmaxf(e, -250.f), 250.f), h = n / 2;
-  return v * pow2i(h) * pow2i(n - h);
+  return make_float2(pow2i(h), pow2i(n - h));
+}
+KIMI_D float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+// Maximum over the 16 lanes of this half of the warp.
+KIMI_D float half_max(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+KIMI_D float half_sum(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
 }
 // The e5m2 parts of two fp16 values: takes the rounding off `h`, exactly.
 KIMI_D uint32_t take_e5m2x2(__half2& h) {
@@ -187,18 +235,20 @@ struct Walk {
 template <typename T, int RH, int QP>
 __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_constant__ TcParams p) {
   using S = Shape<RH, QP>;
-  constexpr int R = S::R;
+  constexpr int R = S::R, HR = RH / 2;  // a thread of a compute group handles HR rows of one token
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = smem_raw + ((1024u - (tc::smem_u32(smem_raw) & 1023u)) & 1023u);  // [slots][kBox]
   uint8_t* sq = ring + (size_t)p.slots * kBox;                // [boxes][NS][128] query parts
-  uint8_t* sp = sq + (size_t)p.boxes * S::NS * 128;           // [2][P_BYTES] weight parts
-  float* sref = reinterpret_cast<float*>(sp + 2 * S::P_BYTES);  // [R] weight references
+  uint8_t* sp = sq + (size_t)p.boxes * S::NS * 128;           // [2][p_bytes] weight parts
+  float4* sfac = reinterpret_cast<float4*>(sp + 2 * p.p_bytes);  // [R] normalisation of a row
+  float* sref = reinterpret_cast<float*>(sfac + R);           // [R] weight references
   float* sreft = sref + R;                                    // [R] sum references
   float* scoef = sreft + R;                                   // [R] score factors
-  float* sred = scoef + R;                                    // [2 kinds][4 warps][R]
+  float* sdel = scoef + R;                                    // [R] change of a weight reference
+  float* smul = sdel + R;                                     // [R] factor of a sum
+  float* sred = smul + R;                                     // [2 kinds][4 warps][R]
   int* slim = reinterpret_cast<int*>(sred + 8 * R);           // [R] keys that a row sees
-  uint64_t* bars = reinterpret_cast<uint64_t*>(slim + R);
-  uint64_t* full = bars;
+  uint64_t* full = reinterpret_cast<uint64_t*>(slim + R);
   uint64_t* empty = full + kMaxSlots;
   uint64_t* s_full = empty + kMaxSlots;
   uint64_t* s_empty = s_full + 2;
@@ -208,81 +258,89 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
   uint64_t* drain = q_full + 1;
   uint32_t* tslot = reinterpret_cast<uint32_t*>(drain + 1);
   int* swalk = reinterpret_cast<int*>(tslot + 1);             // [3] first pair, skip, tiles
+  int* swsum = swalk + 3;                                     // [10] tiles counted by each warp
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int pairs = p.a.batch * p.row_tiles;
   const int width = p.a.cache.width;
 
   // ---- set-up: barriers, TMEM, this CTA's share of the tiles
-  if (tid == 0) {
-    for (int i = 0; i < p.slots; ++i) {
-      tc::mbar_init(&full[i], 1);
-      tc::mbar_init(&empty[i], 1);
-    }
-    for (int i = 0; i < 2; ++i) {
-      tc::mbar_init(&s_full[i], 1);
-      tc::mbar_init(&s_empty[i], 8);
-      tc::mbar_init(&p_full[i], 8);
-      tc::mbar_init(&pv_done[i], 1);
-    }
+  if (warp == 1) tc::tmem_alloc(tslot, p.tmem);
+  if (tid < p.slots) {
+    tc::mbar_init(&full[tid], 1);
+    tc::mbar_init(&empty[tid], 1);
+  }
+  if (tid >= 64 && tid < 66) {
+    tc::mbar_init(&s_full[tid - 64], 1);
+    tc::mbar_init(&s_empty[tid - 64], 8);
+    tc::mbar_init(&p_full[tid - 64], 8);
+    tc::mbar_init(&pv_done[tid - 64], 1);
+  }
+  if (tid == 96) {
     tc::mbar_init(q_full, 8);
     tc::mbar_init(drain, 1);
-    tc::fence_barrier_init();
     tc::tma_prefetch(&p.map);
   }
-  if (warp == 1) tc::tmem_alloc(tslot, p.tmem);
-  if (warp == 0) {
+  {
+    // Every thread counts the tiles of a run of pairs; a block scan places the runs in the tile list.
     int64_t len, start;
     if (p.direct) {
-      const int n = pair_tiles(p, blockIdx.x, &len, &start);
-      if (lane == 0) {
+      if (tid == 0) {
         swalk[0] = blockIdx.x;
         swalk[1] = 0;
-        swalk[2] = n;
+        swalk[2] = pair_tiles(p, blockIdx.x, &len, &start);
       }
     } else {
-      int total = 0;
-      for (int v0 = 0; v0 < pairs; v0 += 32) total += __reduce_add_sync(0xffffffffu, v0 + lane < pairs ? pair_tiles(p, v0 + lane, &len, &start) : 0);
-      const int per = max(p.min_tiles, (total + (int)gridDim.x - 1) / (int)gridDim.x);
-      const int mine = blockIdx.x * per;  // < 2^31: total tiles are bounded by the host
-      int before = 0, first = pairs, skip = 0;
-      for (int v0 = 0; v0 < pairs; v0 += 32) {
-        const int n = v0 + lane < pairs ? pair_tiles(p, v0 + lane, &len, &start) : 0;
-        int incl = n;
+      const int run = (pairs + kThreads - 1) / kThreads, v0 = min(tid * run, pairs), v1 = min(v0 + run, pairs);
+      int own = 0;
+      for (int v = v0; v < v1; ++v) own += pair_tiles(p, v, &len, &start);
+      int incl = own;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int y = __shfl_up_sync(0xffffffffu, incl, o);
-          if (lane >= o) incl += y;
-        }
-        const int at = before + incl - n;
-        if (blockIdx.x == 0 && v0 + lane < pairs) p.prefix[v0 + lane] = at;
-        const unsigned hit = __ballot_sync(0xffffffffu, n > 0 && mine >= at && mine < at + n);
-        if (hit && first == pairs) {
-          first = v0 + __ffs(hit) - 1;
-          skip = mine - __shfl_sync(0xffffffffu, at, __ffs(hit) - 1);
-        }
-        before += __shfl_sync(0xffffffffu, incl, 31);
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
       }
-      if (lane == 0) {
-        swalk[0] = first;
-        swalk[1] = skip;
-        swalk[2] = max(0, min(per, total - mine));
-        if (blockIdx.x == 0) {
-          p.prefix[pairs] = total;
-          p.prefix[pairs + 1] = per;
+      if (lane == 31) swsum[warp] = incl;
+      if (tid == 0) {
+        swalk[0] = pairs;
+        swalk[1] = swalk[2] = 0;
+      }
+      __syncthreads();
+      int at = incl - own, total = 0;
+#pragma unroll
+      for (int i = 0; i < kThreads / 32; ++i) {
+        if (i < warp) at += swsum[i];
+        total += swsum[i];
+      }
+      const int per = max(p.min_tiles, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+      const int mine = blockIdx.x * per;  // < 2^31: the host bounds the number of tiles
+      if (blockIdx.x == 0 || (mine >= at && mine < at + own)) {
+        for (int v = v0; v < v1; ++v) {
+          const int n = run == 1 ? own : pair_tiles(p, v, &len, &start);
+          if (blockIdx.x == 0) p.prefix[v] = at;
+          if (mine >= at && mine < at + n) {
+            swalk[0] = v;
+            swalk[1] = mine - at;
+            swalk[2] = min(per, total - mine);
+          }
+          at += n;
         }
+      }
+      if (blockIdx.x == 0 && tid == 0) {
+        p.prefix[pairs] = total;
+        p.prefix[pairs + 1] = per;
       }
     }
   }
-  // rows of the weight buffers past R stay zero
-  for (int i = tid; i < 2 * S::P_BYTES / 16; i += kThreads) reinterpret_cast<int4*>(sp)[i] = make_int4(0, 0, 0, 0);
-  for (int i = tid; i < p.boxes * S::NS * 8; i += kThreads) reinterpret_cast<int4*>(sq)[i] = make_int4(0, 0, 0, 0);
+  // a context product may read weight parts that no row has: zeros
+  for (int i = tid; i < 2 * p.p_bytes / 16; i += kThreads) reinterpret_cast<int4*>(sp)[i] = make_int4(0, 0, 0, 0);
+  tc::fence_barrier_init();
   tc::fence_proxy_async();
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = *tslot;
-  const uint32_t tm_s = tmem + (uint32_t)(p.boxes * S::NP);  // score buffers behind the accumulators
+  const uint32_t tm_s = tmem + (uint32_t)(p.boxes * p.np);  // score buffers behind the accumulators
   Walk w;
   w.v = swalk[0];
   w.skip = swalk[1];
@@ -293,19 +351,25 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     if (lane == 0) {
       bool ok = true;
       uint32_t n = 0;  // boxes loaded so far
+      int slot = 0;
+      uint32_t ph = 1;  // parity of the last release of `slot` before this use
       while (ok && w.next(p, pairs)) {
         const int b = w.v / p.row_tiles;
-        for (int t = w.t0; ok && t < w.t1; ++t)
+        for (int t = w.t0; ok && t < w.t1; ++t) {
+          const int y = p.t_first ? t * kTile : (int)(b * p.z_mul), z = p.t_first ? (int)(b * p.z_mul) : t * kTile;
           for (int k = 0; k < p.boxes; ++k, ++n) {
-            const uint32_t slot = n % p.slots, use = n / p.slots;
-            if (use > 0 && !tc::mbar_wait(&empty[slot], (use - 1) & 1, p.status, tc::kTimeoutEmpty)) {
+            if (n >= (uint32_t)p.slots && !tc::mbar_wait(&empty[slot], ph, p.status, tc::kTimeoutEmpty)) {
               ok = false;
               break;
             }
             tc::mbar_arrive_expect_tx(&full[slot], kBox);
-            const int y = p.t_first ? t * kTile : (int)(b * p.z_mul), z = p.t_first ? (int)(b * p.z_mul) : t * kTile;
             tc::tma_load_3d(ring + (size_t)slot * kBox, &p.map, &full[slot], k * 128, y, z);
+            if (++slot == p.slots) {
+              slot = 0;
+              ph ^= 1;
+            }
           }
+        }
         ++w.v;
       }
       // copies in flight land before the CTA ends
@@ -313,72 +377,98 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         tc::mbar_wait_local(&full[i % p.slots], (i / p.slots) & 1, p.status, tc::kTimeoutDrain, tc::kDrainNs);
     }
   } else if (warp == 1) {
-    // ---- MMAs
-    if (lane == 0) {
-      bool ok = true;
-      uint32_t n_tile = 0, seg = 0;  // tiles and segments so far
-      constexpr uint32_t id_s = idesc_f8(64, S::NS, false, false);
-      const uint32_t ring0 = tc::smem_u32(ring), q0 = tc::smem_u32(sq), p0 = tc::smem_u32(sp);
-      auto scores = [&](uint32_t g, int k0, int k1) {  // boxes [k0, k1) of tile g's score product
-        const uint32_t buf = g % p.s_bufs, use = g / p.s_bufs;
-        if (k0 == 0) {
-          if (use > 0 && !tc::mbar_wait(&s_empty[buf], (use - 1) & 1, p.status, tc::kTimeoutTmemEmpty)) return false;
-          tc::tc_fence_after();
-        }
-        for (int k = k0; k < k1; ++k) {
-          const uint32_t n = g * p.boxes + k, slot = n % p.slots;
-          if (!tc::mbar_wait(&full[slot], (n / p.slots) & 1, p.status, tc::kTimeoutFull)) return false;
-          tc::tc_fence_after();
+    // ---- MMAs: the whole warp walks, one elected thread issues.  Issued under elect.sync with descriptors
+    // that are sums of precomputed ones, an MMA costs what the tensor core takes (28 clocks for a score
+    // step of 48 columns, 40 for a context step); behind a plain lane test the issue alone took 90 to 170.
+    bool ok = true;
+    uint32_t n_tile = 0, seg = 0;  // tiles and segments so far
+    int s_slot = 0, o_slot = 0;    // next box of the score and of the context stream
+    uint32_t s_ph = 0;
+    const uint32_t id_s = idesc_f8(64, S::NS, false, false), id_o = idesc_f8(128, p.np, true, true);
+    const uint64_t ad_s = tc::smem_desc_sw128(tc::smem_u32(ring), 16, 1024);
+    const uint64_t ad_o = tc::smem_desc_sw128(tc::smem_u32(ring), 8192, 1024);
+    const uint64_t bd_q = tc::smem_desc_sw128(tc::smem_u32(sq), 16, 1024);
+    const uint64_t bd_p = tc::smem_desc_sw128(tc::smem_u32(sp), 16, 1024);
+    auto wait = [&](uint64_t* bar, uint32_t par, int code) {
+      ok = __all_sync(0xffffffffu, ok && tc::mbar_wait(bar, par & 1, p.status, code));
+      tc::tc_fence_after();
+      return ok;
+    };
+    auto scores = [&](uint32_t g, int k0, int k1) {  // boxes [k0, k1) of tile g's score product
+      const uint32_t buf = p.s_bufs == 2 ? g & 1 : 0, use = p.s_bufs == 2 ? g >> 1 : g;
+      if (k0 == 0 && use > 0 && !wait(&s_empty[buf], use - 1, tc::kTimeoutTmemEmpty)) return;
+      for (int k = k0; k < k1; ++k) {
+        if (!wait(&full[s_slot], s_ph, tc::kTimeoutFull)) return;
+        if (elect_one()) {
+          const uint64_t ad = ad_s + (uint64_t)(s_slot * (kBox >> 4)), bd = bd_q + (uint64_t)(k * S::NS * 8);
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            mma_f8(tm_s + buf * S::NS, tc::smem_desc_sw128(ring0 + slot * kBox + j * 32, 16, 1024),
-                   tc::smem_desc_sw128(q0 + k * S::NS * 128 + j * 32, 16, 1024), id_s, (k | j) != 0);
+          for (int j = 0; j < 4; ++j) mma_f8(tm_s + buf * S::NS, ad + 2 * j, bd + 2 * j, id_s, (k | j) != 0);
+          if (k == p.boxes - 1) tc::mma_commit(&s_full[buf]);
         }
-        if (k1 == p.boxes && k0 < k1) tc::mma_commit(&s_full[buf]);
-        return true;
-      };
-      while (ok && w.next(p, pairs)) {
-        if (!tc::mbar_wait(q_full, seg & 1, p.status, tc::kTimeoutTmemEmpty)) break;
-        tc::tc_fence_after();
-        ok = scores(n_tile, 0, p.boxes);
-        for (int t = w.t0; ok && t < w.t1; ++t, ++n_tile) {
-          const bool more = t + 1 < w.t1;
-          if (more && p.ahead > 0 && !(ok = scores(n_tile + 1, 0, p.ahead))) break;
-          const uint32_t pb = n_tile & 1;
-          if (!(ok = tc::mbar_wait(&p_full[pb], (n_tile >> 1) & 1, p.status, tc::kTimeoutTmemFull))) break;
-          tc::tc_fence_after();
-          for (int k = 0; k < p.boxes; ++k) {
-            const uint32_t slot = (n_tile * p.boxes + k) % p.slots;
-#pragma unroll
-            for (int part = 0; part < S::WP; ++part)
-#pragma unroll
-              for (int j = 0; j < 2; ++j)
-                mma_f8(tmem + (uint32_t)(k * S::NP), tc::smem_desc_sw128(ring0 + slot * kBox + j * 4096, 8192, 1024),
-                       tc::smem_desc_sw128(p0 + pb * S::P_BYTES + (part >> 1) * S::NP * 128 + (part & 1) * 64 + j * 32, 16, 1024),
-                       idesc_f8(128, S::NP, true, true), (t > w.t0 || part > 0 || j > 0) ? 1u : 0u);
-            tc::mma_commit(&empty[slot]);
-          }
-          tc::mma_commit(&pv_done[pb]);
-          if (more && p.ahead < p.boxes) ok = scores(n_tile + 1, p.ahead, p.boxes);
+        __syncwarp();
+        if (++s_slot == p.slots) {
+          s_slot = 0;
+          s_ph ^= 1;
         }
-        ++seg;
-        ++w.v;
       }
+    };
+    while (ok && w.next(p, pairs)) {
+      if (!wait(q_full, seg, tc::kTimeoutTmemEmpty)) break;
+      scores(n_tile, 0, p.boxes);
+      for (int t = w.t0; ok && t < w.t1; ++t, ++n_tile) {
+        const bool more = t + 1 < w.t1;
+        if (more && p.ahead > 0) scores(n_tile + 1, 0, p.ahead);
+        const uint32_t pb = n_tile & 1;
+        if (!ok || !wait(&p_full[pb], n_tile >> 1, tc::kTimeoutTmemFull)) break;
+        for (int k = 0; k < p.boxes; ++k) {
+          if (elect_one()) {
+            const uint64_t ad = ad_o + (uint64_t)(o_slot * (kBox >> 4)), bd = bd_p + (uint64_t)(pb * (p.p_bytes >> 4));
+            const uint32_t d = tmem + (uint32_t)(k * p.np);
+            for (int run = 0; run < p.runs; ++run) {
+              const uint64_t br = bd + (uint64_t)((run >> 1) * p.np * 8 + (run & 1) * 4);
+              mma_f8(d, ad, br, id_o, (t > w.t0 || run > 0) ? 1u : 0u);
+              mma_f8(d, ad + (4096 >> 4), br + 2, id_o, 1u);
+            }
+            tc::mma_commit(&empty[o_slot]);
+            if (k == p.boxes - 1) tc::mma_commit(&pv_done[pb]);
+          }
+          __syncwarp();
+          if (++o_slot == p.slots) o_slot = 0;
+        }
+        if (more && p.ahead < p.boxes) scores(n_tile + 1, p.ahead, p.boxes);
+      }
+      ++seg;
+      ++w.v;
+    }
+    if (elect_one()) {
       tc::mma_commit(drain);
       tc::mbar_wait_local(drain, 0, p.status, tc::kTimeoutDrain, tc::kDrainNs);
     }
+    __syncwarp();
   } else {
-    // ---- compute groups: rows [grp * RH, grp * RH + RH) of the pair
+    // ---- compute groups: rows [grp * RH, grp * RH + RH) of the pair.  The score tile has M = 64: its tokens
+    // lie in lanes 0-15 of each warp's quadrant, and the halves of a warp take half of the rows each.
     const int grp = (warp - 2) >> 2, quad = warp & 3, bar_id = 1 + grp, cw = warp - 2;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-    const int tok = quad * 16 + (lane & 15);  // score lanes 0-15 of each quadrant hold the 64 tokens
-    const bool active = lane < 16;
-    const int r0 = grp * RH;
-    float* red = sred + quad * R;  // [2][4][R]
+    const int tok = quad * 16 + (lane & 15);
+    const int r0 = grp * RH, rr = r0 + (lane >> 4) * HR;  // rows of the group and of this thread
+    // weight parts: run `part / stack` takes 64 bytes of a 128-byte row, stacked parts take R rows each
+    uint32_t part_at[S::WP], row_at[HR];
+#pragma unroll
+    for (int i = 0; i < S::WP; ++i) {
+      const int run = i / p.stack, g = i - run * p.stack;
+      part_at[i] = (uint32_t)((run >> 1) * p.np * 128 + g * R * 128) | ((run & 1) << 31);
+    }
+#pragma unroll
+    for (int r = 0; r < HR; ++r) {
+      const int n = rr + r;
+      row_at[r] = (uint32_t)((n >> 3) * 1024 + (n & 7) * 128 + ((quad ^ (n & 7)) << 4) + (lane & 15));
+    }
     // A wait that fails only makes this warp skip its later waits: every warp walks all tiles, so the
     // groups' named barriers always meet and the kernel ends (its results are void, as the status says).
     bool ok = true;
     uint32_t n_tile = 0;
+    int slot = 0;  // first box of the tile
     auto wait = [&](uint64_t* bar, uint32_t use, int code) {  // the warp is converged again behind it
       ok = ok && tc::mbar_wait(bar, use & 1, p.status, code);
       __syncwarp();
@@ -387,173 +477,219 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     while (w.next(p, pairs)) {
       const int b = w.v / p.row_tiles, row0 = (w.v - b * p.row_tiles) * p.rows_tile;
       const int nrow = min(p.rows_tile, p.rows - row0);
-      // -- query rows into parts; one warp per row
-      for (int r = cw; r < nrow; r += 8) {
-        const int qi = (row0 + r) / p.a.heads, h = (row0 + r) - qi * p.a.heads;
+      // -- query rows into parts; one warp per row, the second read of a row comes from L1
+#pragma unroll 1
+      for (int r = cw; r < R; r += 8) {
+        const int qr = row0 + min(r, nrow - 1), qi = qr / p.a.heads, h = qr - qi * p.a.heads;
         const T* q = static_cast<const T*>(p.a.q) + b * p.a.q_b + qi * p.a.q_i + h * p.a.q_h;
+        const int64_t seen = w.start + qi + 1;
+        if (lane == 0) {
+          slim[r] = seen < 0 ? 0 : (int)(seen < w.len ? seen : w.len);
+          sref[r] = sreft[r] = -INFINITY;
+          scoef[r] = 0.f;
+        }
+        if (r >= nrow) continue;
+        const int octs = width >> 3;
+        auto load = [&](int o) {
+          int4 x = make_int4(0, 0, 0, 0);
+          if (o < octs) {
+            if (p.q_vec) {
+              x = __ldg(reinterpret_cast<const int4*>(q) + o);
+            } else {
+              Vec<T> e;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) e.v[j] = q[o * 8 + j];
+              x = *reinterpret_cast<const int4*>(e.v);
+            }
+          }
+          return x;
+        };
         uint32_t top = 0;
-        for (int l = lane; l < width; l += 32) top = max(top, __float_as_uint(to_f<T>(q[l])) & 0x7FFFFFFFu);
-        top = __reduce_max_sync(0xffffffffu, top);
+#pragma unroll
+        for (int i = 0; i < kOcts; ++i) {
+          const int4 x = load(lane + 32 * i);
+          const uint32_t m = 0x7FFF7FFFu;
+          top = __vmaxu2(__vmaxu2(top, __vmaxu2(x.x & m, x.y & m)), __vmaxu2(x.z & m, x.w & m));
+        }
+        top = __reduce_max_sync(0xffffffffu, max(top & 0xFFFFu, top >> 16));
+        const unsigned short top16 = (unsigned short)top;
+        top = __float_as_uint(to_f<T>(*reinterpret_cast<const T*>(&top16)));
         const bool bad = top >= 0x7F800000u;
         const int k = bad ? 0 : min(126, 134 - (int)(top >> 23));  // the maximum to [128, 256)
-        const float f = bad ? 0.f : pow2i(k);
-        for (int l = lane; l < p.boxes * 128; l += 32) {
-          float x = l < width && !bad ? to_f<T>(q[l]) * f : 0.f;
+        const float f = pow2i(k);
+#pragma unroll 1
+        for (int o = lane; o < p.boxes * 16; o += 32) {
+          Vec<T> e;
+          *reinterpret_cast<int4*>(e.v) = load(o);
+          float v[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = bad ? 0.f : e.f(j) * f;
+          uint8_t* at = sq + (size_t)(o >> 4) * S::NS * 128 + (o & 1) * 8;
 #pragma unroll
           for (int part = 0; part < QP; ++part) {
             const int n = part * R + r;
-            const uint8_t c = (uint8_t)to_codes2(x, 0.f);
-            sq[(size_t)(l >> 7) * S::NS * 128 + (n >> 3) * 1024 + (n & 7) * 128 + ((((l >> 4) & 7) ^ (n & 7)) << 4) + (l & 15)] = c;
-            x = (x - code1(c)) * 32.f;
+            uint32_t c[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              c[j] = to_codes2(v[2 * j], v[2 * j + 1]);
+              const float2 d = codes2(c[j]);
+              v[2 * j] = (v[2 * j] - d.x) * 32.f;
+              v[2 * j + 1] = (v[2 * j + 1] - d.y) * 32.f;
+            }
+            *reinterpret_cast<uint2*>(at + (n >> 3) * 1024 + (n & 7) * 128 + ((((o >> 1) & 7) ^ (n & 7)) << 4)) =
+                make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
           }
         }
         if (lane == 0) scoef[r] = bad ? __uint_as_float(0x7FC00000u) : p.a.scale * kLog2e * pow2i(-k);
       }
-      if (cw == 0)
-        for (int r = lane; r < R; r += 32) {
-          const int64_t seen = w.start + (row0 + r) / p.a.heads + 1;
-          slim[r] = r >= nrow || seen < 0 ? 0 : (int)(seen < w.len ? seen : w.len);
-          sref[r] = -INFINITY;
-          sreft[r] = -INFINITY;
-          if (r >= nrow) scoef[r] = 0.f;
-        }
       tc::fence_proxy_async();
       tc::tc_fence_before();
       __syncwarp();
       asm volatile("bar.sync 3, 256;\n" ::: "memory");
       if (lane == 0) tc::mbar_arrive(q_full);
-      float sum[RH];
+      const int lim0 = slim[0];  // rows come in the order of their positions
+      float sum[HR];
 #pragma unroll
-      for (int r = 0; r < RH; ++r) sum[r] = 0.f;
+      for (int r = 0; r < HR; ++r) sum[r] = 0.f;
       const float* scales = p.a.cache.scales + b * p.a.cache.scale_b;
       for (int t = w.t0; t < w.t1; ++t, ++n_tile) {
         const int at = t * kTile + tok;
-        const float st = active && at < w.len ? scales[at * p.a.cache.scale_t] : 0.f;
-        const float lg = log2f(st);
-        const uint32_t buf = n_tile % p.s_bufs, pb = n_tile & 1;
-        wait(&s_full[buf], n_tile / p.s_bufs, tc::kTimeoutTmemFull);
-        float s[RH];
+        const float st = at < w.len ? scales[at * p.a.cache.scale_t] : 0.f;
+        const uint32_t buf = p.s_bufs == 2 ? n_tile & 1 : 0, pb = n_tile & 1;
+        wait(&s_full[buf], p.s_bufs == 2 ? n_tile >> 1 : n_tile, tc::kTimeoutTmemFull);
+        float s[HR];
         {
-          float v[QP][RH];
+          float v[QP][HR];
 #pragma unroll
           for (int part = 0; part < QP; ++part)
-#pragma unroll
-            for (int r = 0; r < RH; r += 4) tmem_ld4(tm_s + lanes + buf * S::NS + part * R + r0 + r, v[part] + r);
+            tmem_ld_halves<HR, HR>(tm_s + lanes + buf * S::NS + part * R + r0, v[part]);
           tmem_wait_ld();
 #pragma unroll
-          for (int r = 0; r < RH; ++r) {
+          for (int r = 0; r < HR; ++r) {
             float x = v[QP - 1][r];
 #pragma unroll
             for (int part = QP - 2; part >= 0; --part) x = fmaf(x, 0.03125f, v[part][r]);
-            s[r] = x;
+            s[r] = x * (scoef[rr + r] * st);
           }
         }
         tc::tc_fence_before();
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(&s_empty[buf]);
-        // slots past the length hold anything: their rows of the tile become zeros
-        if ((int64_t)(t + 1) * kTile > w.len) {
-          const int from = (int)(w.len - (int64_t)t * kTile), n = (kTile - from) * 8;
-          for (int k = 0; k < p.boxes; ++k) {
-            uint8_t* box = ring + (size_t)((n_tile * p.boxes + k) % p.slots) * kBox + from * 128;
-            for (int i = tid - 64; i < n; i += 256) reinterpret_cast<int4*>(box)[i] = make_int4(0, 0, 0, 0);
+        const float lg = log2f(st);
+        uint32_t see = 0xFFFFFFFFu;
+        if ((t + 1) * kTile > lim0) {  // a tile that some row does not see whole
+          see = 0;
+#pragma unroll
+          for (int r = 0; r < HR; ++r) see |= (at < slim[rr + r] ? 1u : 0u) << r;
+          // slots past the length hold anything: their rows of the tile become zeros
+          if ((int64_t)(t + 1) * kTile > w.len) {
+            const int from = (int)(w.len - (int64_t)t * kTile), n = (kTile - from) * 8;
+            for (int k = 0, i = slot; k < p.boxes; ++k) {
+              uint8_t* box = ring + (size_t)i * kBox + from * 128;
+              for (int j = tid - 64; j < n; j += 256) reinterpret_cast<int4*>(box)[j] = make_int4(0, 0, 0, 0);
+              if (++i == p.slots) i = 0;
+            }
           }
         }
+        slot += p.boxes;
+        if (slot >= p.slots) slot -= p.slots;
         bool raise = false;
-        uint32_t see = 0;
 #pragma unroll
-        for (int r = 0; r < RH; ++r) {
-          s[r] *= scoef[r0 + r] * st;
-          const bool on = active && at < slim[r0 + r];
-          see |= (on ? 1u : 0u) << r;
-          raise |= on && (s[r] + lg > sref[r0 + r] + kTop || s[r] > sreft[r0 + r] + kSumRoom);
-        }
+        for (int r = 0; r < HR; ++r)
+          raise |= ((see >> r) & 1) && (s[r] + lg > sref[rr + r] + kTop || s[r] > sreft[rr + r] + kSumRoom);
         __syncwarp();
         if (group_any(bar_id, raise)) {
-          // some row outgrew its reference: new ones from the tile's maxima
+          // some row outgrew a reference: new ones from the tile's maxima
 #pragma unroll
-          for (int r = 0; r < RH; ++r) {
-            float ma = (see >> r) & 1 ? s[r] + lg : -INFINITY, ms = (see >> r) & 1 ? s[r] : -INFINITY;
-            ma = warp_max(ma);
-            ms = warp_max(ms);
-            if (lane == 0) {
-              red[r0 + r] = ma;
-              red[4 * R + r0 + r] = ms;
+          for (int r = 0; r < HR; ++r) {
+            const bool on = (see >> r) & 1;
+            const float ma = half_max(on ? s[r] + lg : -INFINITY), ms = half_max(on ? s[r] : -INFINITY);
+            if ((lane & 15) == 0) {
+              sred[quad * R + rr + r] = ma;
+              sred[(4 + quad) * R + rr + r] = ms;
             }
           }
-          group_sync(bar_id);
-          bool waited = false;
-#pragma unroll
-          for (int r = 0; r < RH; ++r) {
-            float ma = -INFINITY, ms = -INFINITY;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              ma = fmaxf(ma, sred[q * R + r0 + r]);
-              ms = fmaxf(ms, sred[(4 + q) * R + r0 + r]);
-            }
-            if (ms > sreft[r0 + r] + kSumRoom) sum[r] *= exp2f(sreft[r0 + r] - ceilf(ms));
-            if (t > w.t0 && ma > sref[r0 + r] + kTop) {  // uniform over the group
-              if (!waited) {
-                wait(&pv_done[pb ^ 1], (n_tile - 1) >> 1, tc::kTimeoutTmemEmpty);
-                waited = true;
-              }
-              const float d = sref[r0 + r] - (ceilf(ma) - (kTop - kRoom));
-              for (int k = 0; k < p.boxes; ++k) {
-                const uint32_t c = tmem + lanes + (uint32_t)(k * S::NP + r0 + r);
-                float v = tmem_ld1(c);
-                tmem_wait_ld();
-                tmem_st1(c, d == -INFINITY ? 0.f : scale2(v, d));
-              }
-            }
-          }
-          if (waited) tmem_wait_st();
           group_sync(bar_id);
           if (quad == 0 && lane < RH) {
-            float ma = -INFINITY, ms = -INFINITY;
-            for (int q = 0; q < 4; ++q) {
-              ma = fmaxf(ma, sred[q * R + r0 + lane]);
-              ms = fmaxf(ms, sred[(4 + q) * R + r0 + lane]);
+            const int r = r0 + lane;
+            const float ma = fmaxf(fmaxf(sred[r], sred[R + r]), fmaxf(sred[2 * R + r], sred[3 * R + r]));
+            const float ms = fmaxf(fmaxf(sred[4 * R + r], sred[5 * R + r]), fmaxf(sred[6 * R + r], sred[7 * R + r]));
+            float del = 0.f, mul = 1.f;
+            if (ma > sref[r] + kTop) {
+              const float to = ceilf(ma) - (kTop - kRoom);
+              del = sref[r] - to;
+              sref[r] = to;
             }
-            if (ma > sref[r0 + lane] + kTop) sref[r0 + lane] = ceilf(ma) - (kTop - kRoom);
-            if (ms > sreft[r0 + lane] + kSumRoom) sreft[r0 + lane] = ceilf(ms);
+            if (ms > sreft[r] + kSumRoom) {
+              const float to = ceilf(ms);
+              mul = exp2f(sreft[r] - to);
+              sreft[r] = to;
+            }
+            sdel[r] = del;
+            smul[r] = mul;
           }
           group_sync(bar_id);
+#pragma unroll
+          for (int r = 0; r < HR; ++r) sum[r] *= smul[rr + r];
+          if (t > w.t0) {  // the accumulators hold something
+            bool waited = false;
+#pragma unroll 1
+            for (int r = r0; r < r0 + RH; ++r) {
+              const float del = sdel[r];
+              if (del == 0.f) continue;  // uniform over the group
+              if (!waited) wait(&pv_done[pb ^ 1], (n_tile - 1) >> 1, tc::kTimeoutTmemEmpty);
+              waited = true;
+              const float2 f = del == -INFINITY ? make_float2(0.f, 0.f) : pow2_pair(del);
+#pragma unroll 1
+              for (int g = 0; g < p.stack; ++g) {
+                const uint32_t c = tmem + lanes + (uint32_t)(g * R + r);
+#pragma unroll 1
+                for (int k = 0; k < p.boxes; k += 4) {
+                  float v[4];
+#pragma unroll
+                  for (int i = 0; i < 4; ++i)
+                    if (k + i < p.boxes) v[i] = tmem_ld1(c + (uint32_t)((k + i) * p.np));
+                  tmem_wait_ld();
+#pragma unroll
+                  for (int i = 0; i < 4; ++i)
+                    if (k + i < p.boxes) tmem_st1(c + (uint32_t)((k + i) * p.np), v[i] * f.x * f.y);
+                }
+              }
+            }
+            if (waited) tmem_wait_st();
+          }
         }
         // weights into parts; the buffer was last read by the context product of two tiles ago
         if (n_tile >= 2) wait(&pv_done[pb], (n_tile >> 1) - 1, tc::kTimeoutTmemEmpty);
-        uint8_t* wp = sp + pb * S::P_BYTES + (tok & 15);
+        uint8_t* wp = sp + pb * p.p_bytes;
 #pragma unroll
-        for (int r = 0; r < RH; r += 2) {
+        for (int r = 0; r < HR; r += 2) {
           float v[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const float x = s[r + e], ax = x + lg;
             const bool on = (see >> (r + e)) & 1;
             // a score of -inf weighs nothing, also against a reference of -inf
-            sum[r + e] += on && x != -INFINITY ? exp2f(x - sreft[r0 + r + e]) : 0.f;
-            v[e] = on && ax != -INFINITY ? exp2f(ax - sref[r0 + r + e]) : 0.f;
+            sum[r + e] += on && x != -INFINITY ? ex2(x - sreft[rr + r + e]) : 0.f;
+            v[e] = on && ax != -INFINITY ? ex2(ax - sref[rr + r + e]) : 0.f;
           }
-          if (active) {
-            // fp16 holds three parts; with four, the first comes off in fp32
-            __half2 h;
-            if constexpr (S::WP == 3) h = __floats2half2_rn(v[0], v[1]);
+          // fp16 holds three parts; with four, the first comes off in fp32
+          __half2 h;
+          if constexpr (S::WP == 3) h = __floats2half2_rn(v[0], v[1]);
 #pragma unroll
-            for (int part = 0; part < S::WP; ++part) {
-              uint32_t c;
-              if (S::WP > 3 && part == 0) {
-                c = __nv_cvt_float2_to_fp8x2(make_float2(v[0], v[1]), __NV_SATFINITE, __NV_E5M2);
-                const float2 d = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)c, __NV_E5M2)));
-                h = __floats2half2_rn(v[0] - d.x, v[1] - d.y);
-              } else {
-                c = take_e5m2x2(h);
-              }
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int n = r0 + r + e;
-                wp[(part >> 1) * S::NP * 128 + (n >> 3) * 1024 + (n & 7) * 128 + ((((part & 1) * 4 + quad) ^ (n & 7)) << 4)] =
-                    (uint8_t)(c >> (8 * e));
-              }
+          for (int part = 0; part < S::WP; ++part) {
+            uint32_t c;
+            if (S::WP > 3 && part == 0) {
+              c = __nv_cvt_float2_to_fp8x2(make_float2(v[0], v[1]), __NV_SATFINITE, __NV_E5M2);
+              const float2 d = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)c, __NV_E5M2)));
+              h = __floats2half2_rn(v[0] - d.x, v[1] - d.y);
+            } else {
+              c = take_e5m2x2(h);
             }
+            uint8_t* to = wp + (part_at[part] & 0x7FFFFFFFu);
+            const uint32_t flip = (part_at[part] >> 31) << 6;  // the row's other 64 bytes
+            to[row_at[r] ^ flip] = (uint8_t)c;
+            to[row_at[r + 1] ^ flip] = (uint8_t)(c >> 8);
           }
         }
         tc::fence_proxy_async();
@@ -562,40 +698,51 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         if (lane == 0) tc::mbar_arrive(&p_full[pb]);
       }
       // -- epilogue: normalise, write the output or this CTA's part of it
-      const uint32_t last = n_tile - 1;
 #pragma unroll
-      for (int r = 0; r < RH; ++r) {
-        const float x = warp_sum(sum[r]);  // idle lanes hold 0
-        if (lane == 0) red[r0 + r] = x;
+      for (int r = 0; r < HR; ++r) {
+        const float x = half_sum(sum[r]);
+        if ((lane & 15) == 0) sred[quad * R + rr + r] = x;
       }
       group_sync(bar_id);
       const bool whole = w.t0 == 0 && w.t1 == w.tiles;
-      const int64_t slot = (int64_t)blockIdx.x + w.v;
-      float inv[RH];
-#pragma unroll
-      for (int r = 0; r < RH; ++r) {
-        const float x = sred[r0 + r] + sred[R + r0 + r] + sred[2 * R + r0 + r] + sred[3 * R + r0 + r];
-        inv[r] = x != 0.f ? 1.f / x : 0.f;
-        if (!whole && quad == 0 && lane == 0 && r0 + r < nrow)
-          p.part_lse[slot * p.rows_tile + r0 + r] = x != 0.f ? sreft[r0 + r] + log2f(x) : -INFINITY;
+      const int64_t part = (int64_t)blockIdx.x + w.v;
+      if (quad == 0 && lane < RH) {
+        const int r = r0 + lane;
+        const float x = sred[r] + sred[R + r] + sred[2 * R + r] + sred[3 * R + r];
+        // no key: the row is zeros; references are finite otherwise (or the row is NaN)
+        const float2 f = x != 0.f ? pow2_pair(sref[r] - sreft[r]) : make_float2(0.f, 0.f);
+        sfac[r] = make_float4(f.x, f.y, x != 0.f ? 1.f / x : 0.f, 0.f);
+        if (!whole && r < nrow) p.part_lse[part * p.rows_tile + r] = x != 0.f ? sreft[r] + log2f(x) : -INFINITY;
       }
-      wait(&pv_done[last & 1], last >> 1, tc::kTimeoutTmemEmpty);
+      group_sync(bar_id);
+      wait(&pv_done[(n_tile - 1) & 1], (n_tile - 1) >> 1, tc::kTimeoutTmemEmpty);
+      const int64_t first = whole ? (int64_t)b * p.rows + row0 + r0 : part * p.rows_tile + r0;
+#pragma unroll 1
       for (int k = 0; k < p.boxes; ++k) {
         float v[RH];
 #pragma unroll
-        for (int r = 0; r < RH; r += 4) tmem_ld4(tmem + lanes + (uint32_t)(k * S::NP + r0 + r), v + r);
+        for (int r = 0; r < RH; r += 4) tmem_ld4(tmem + lanes + (uint32_t)(k * p.np + r0 + r), v + r);
         tmem_wait_ld();
+#pragma unroll 1
+        for (int g = 1; g < p.stack; ++g) {
+          float x[RH];
+#pragma unroll
+          for (int r = 0; r < RH; r += 4) tmem_ld4(tmem + lanes + (uint32_t)(k * p.np + g * R + r0 + r), x + r);
+          tmem_wait_ld();
+#pragma unroll
+          for (int r = 0; r < RH; ++r) v[r] += x[r];
+        }
         const int l = k * 128 + quad * 32 + lane;
         if (l < width) {
+          const int64_t at = first * width + l;
 #pragma unroll
           for (int r = 0; r < RH; ++r) {
-            if (r0 + r >= nrow) continue;
-            // inv == 0: no key (the accumulator may hold a stale column); references are finite otherwise
-            const float o = inv[r] == 0.f ? 0.f : scale2(v[r], sref[r0 + r] - sreft[r0 + r]) * inv[r];
-            if (whole)
-              static_cast<T*>(p.a.out)[((int64_t)b * p.rows + row0 + r0 + r) * width + l] = from_f<T>(o);
-            else
-              p.part_o[(slot * p.rows_tile + r0 + r) * width + l] = o;
+            if (r0 + r < nrow) {
+              const float4 f = sfac[r0 + r];
+              const float o = f.z == 0.f ? 0.f : v[r] * f.x * f.y * f.z;
+              if (whole) static_cast<T*>(p.a.out)[at + (int64_t)r * width] = from_f<T>(o);
+              else p.part_o[at + (int64_t)r * width] = o;
+            }
           }
         }
       }
@@ -645,26 +792,43 @@ __global__ void __launch_bounds__(256) attn_tc_join_kernel(const __grid_constant
   }
 }
 
+// Weight parts on N cost accumulator columns, parts along K cost a pass over the tile (36 + N / 5 clocks
+// per 32 tokens x 128 latents as measured, whatever N holds): as many on N as make the passes cheapest.
 template <int RH, int QP>
 bool fit(int boxes, Plan* pl) {
   using S = Shape<RH, QP>;
-  const int o_cols = boxes * S::NP;
-  const int bufs = o_cols + 2 * S::NS <= 512 ? 2 : o_cols + S::NS <= 512 ? 1 : 0;
-  const size_t fixed = (size_t)boxes * S::NS * 128 + 2 * S::P_BYTES + (3 + 8 + 1) * S::R * 4 + (2 * kMaxSlots + 10) * 8 + 64 + 1024;
-  if (!bufs || fixed >= kSmemMax) return false;
-  int slots = (int)((kSmemMax - fixed) / kBox);
-  slots = slots < kMaxSlots ? slots : kMaxSlots;
-  if (slots < boxes + 2) return false;  // a tile and something to load meanwhile
-  pl->rh = RH;
-  pl->boxes = boxes;
-  pl->slots = slots;
-  pl->s_bufs = bufs;
-  pl->ahead = slots - boxes < boxes ? slots - boxes : boxes;
-  uint32_t cols = 32;
-  while (cols < (uint32_t)(o_cols + bufs * S::NS)) cols *= 2;
-  pl->tmem = cols;
-  pl->smem = fixed + (size_t)slots * kBox;
-  return true;
+  bool found = false;
+  int best = 0;
+  for (int stack = 1; stack <= S::WP; ++stack) {
+    const int np = pad16(stack * S::R), runs = (S::WP + stack - 1) / stack, cols = boxes * np;
+    const int bufs = cols + 2 * S::NS <= 512 ? 2 : cols + S::NS <= 512 ? 1 : 0;
+    if (np > 256 || !bufs || (found && bufs < pl->s_bufs)) continue;
+    const int cost = runs * (36 * 5 + np);
+    if (found && cost >= best && bufs <= pl->s_bufs) continue;
+    const int p_bytes = np * 128 * ((runs + 1) / 2);
+    const size_t fixed = (size_t)boxes * S::NS * 128 + 2 * p_bytes + (4 + 5 + 8 + 1) * S::R * 4 +
+                         (2 * kMaxSlots + 10) * 8 + 64 + 1024;  // + alignment
+    if (fixed >= kSmemMax) continue;
+    int slots = (int)((kSmemMax - fixed) / kBox);
+    slots = slots < kMaxSlots ? slots : kMaxSlots;
+    if (slots < boxes + 2) continue;  // a tile and something to load meanwhile
+    found = true;
+    best = cost;
+    pl->rh = RH;
+    pl->boxes = boxes;
+    pl->slots = slots;
+    pl->s_bufs = bufs;
+    pl->stack = stack;
+    pl->runs = runs;
+    pl->np = np;
+    pl->p_bytes = p_bytes;
+    pl->ahead = slots - boxes < boxes ? slots - boxes : boxes;
+    uint32_t n = 32;
+    while (n < (uint32_t)(cols + bufs * S::NS)) n *= 2;
+    pl->tmem = n;
+    pl->smem = fixed + (size_t)slots * kBox;
+  }
+  return found;
 }
 
 // Rows of a CTA: the fewest padded rows that hold them all, else as many as fit TMEM and shared memory
@@ -767,7 +931,7 @@ cudaError_t launch_rh(const TcParams& p, const Plan& pl, cudaStream_t s) {
 // 16-bit queries, and code rows that TMA can address: 16-byte base and strides.
 bool mla_attn_tc_supported(int dtype, const MlaCacheAttnArgs& a) {
   if (dtype != 1 && dtype != 2) return false;
-  if (a.cache.width % 16 || a.cache.width < 64 || a.cache.slots > (1 << 30)) return false;
+  if (a.cache.width % 16 || a.cache.width < 64 || a.cache.width > 256 * kOcts || a.cache.slots > (1 << 30)) return false;
   if ((reinterpret_cast<uintptr_t>(a.cache.codes) & 15) || (a.batch > 1 && a.cache.code_b % 16)) return false;
   if (a.cache.slots > 1 && (a.cache.code_t % 16 || a.cache.code_t < a.cache.width)) return false;
   Plan pl;
@@ -794,8 +958,13 @@ cudaError_t mla_attn_tc(int dtype, const MlaCacheAttnArgs& a, cudaStream_t s) {
   p.slots = pl.slots;
   p.s_bufs = pl.s_bufs;
   p.ahead = pl.ahead;
+  p.stack = pl.stack;
+  p.runs = pl.runs;
+  p.np = pl.np;
+  p.p_bytes = pl.p_bytes;
   p.direct = pl.direct ? 1 : 0;
   p.min_tiles = 1;
+  p.q_vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.q_b % 8 == 0 && a.q_i % 8 == 0 && a.q_h % 8 == 0;
   p.tmem = pl.tmem;
   const bool one = a.batch == 1 || a.cache.code_b == 0;  // every sequence reads the same rows
   p.z_mul = one ? 0 : 1;
