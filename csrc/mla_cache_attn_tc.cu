@@ -32,8 +32,13 @@
 // a captured graph) needs no lengths on the host.  A CTA that has a whole pair writes its output; the
 // others leave a normalised context and its log-sum, joined by a second kernel in a fixed order.
 //
-// Roles of a CTA (10 warps): warp 0 loads, warp 1 issues the MMAs, warps 2-9 are two groups of four
-// that share the rows: scores -> weights, rescaling, query preparation and the epilogue.
+// Three launches, each started while the one before still runs (programmatic dependent launch): the
+// query parts and the split of the tile list; the attention; the join.  The query parts are written as
+// the image of their shared-memory tile, so that a CTA brings in the next sequence's queries with one
+// bulk copy while it still works on the last tile of this one.
+//
+// Roles of an attention CTA (10 warps): warp 0 loads, warp 1 issues the MMAs, warps 2-9 are two groups
+// of four that share the rows: scores -> weights, rescaling and the epilogue.
 // Every mbarrier wait is bounded and reports through the status word.
 #include <cudaTypedefs.h>
 
@@ -52,7 +57,8 @@ using namespace mlac;
 constexpr int kTile = 64;                  // tokens of a tile
 constexpr int kBox = kTile * 128;          // bytes of a box
 constexpr int kThreads = 320;
-constexpr int kMaxSlots = 32;              // ring slots
+constexpr int kMaxStages = 32;             // of the ring
+constexpr int kMaxGroup = 6;               // boxes of a stage
 constexpr int kSmemMax = 227 * 1024;
 constexpr int kOcts = 8;                   // 8-element pieces of a query row per lane: widths up to 2,048
 constexpr float kTop = 15.f;               // a weight may reach 2^kTop
@@ -64,13 +70,15 @@ struct Plan {
   int rows_tile = 0;   // rows of a pair (<= 2 * rh)
   int row_tiles = 0;
   int boxes = 0;       // boxes of a tile: ceil(L / 128)
-  int slots = 0;       // ring slots
+  int group = 0;       // boxes of a ring stage: one wait, one release
+  int tile_stages = 0;  // stages of a tile
+  int stages = 0;      // of the ring
   int s_bufs = 0;
   int stack = 0;       // weight parts side by side on N
   int runs = 0;        // context products of a box: ceil(parts / stack)
-  int np = 0;          // N of the context product
+  int ns = 0, np = 0;  // N of the score and of the context product
   int p_bytes = 0;     // one weight buffer
-  int ahead = 0;       // boxes of the next tile's scores issued before this tile's context product
+  int ahead = 0;       // stages of the next tile's scores issued before this tile's context product
   uint32_t tmem = 0;
   size_t smem = 0;
   bool direct = false;  // one CTA per pair, nothing to join
@@ -80,13 +88,16 @@ struct Plan {
 struct TcParams {
   CUtensorMap map;
   MlaCacheAttnArgs a;
-  int rows, rows_tile, row_tiles, boxes, slots, s_bufs, ahead, direct, min_tiles, t_first, q_vec;
-  int stack, runs, np, p_bytes;
+  int rows, rows_tile, row_tiles, boxes, group, tile_stages, stages, s_bufs, ahead, direct, min_tiles, t_first, q_vec;
+  int r_pad, stack, runs, ns, np, p_bytes, q_bytes, grid;
   uint32_t tmem;
   int64_t z_mul;       // 0 when every sequence reads the same cache rows
+  uint8_t* q_parts;    // [pairs][q_bytes]: the shared-memory image of a pair's query parts
+  float* coef;         // [pairs][R] score factors
   float* part_o;       // [grid + pairs][rows_tile][L]
   float* part_lse;     // [grid + pairs][rows_tile]
   int* prefix;         // [pairs + 2]: first tile of each pair, total, tiles per CTA
+  int* first;          // [grid][2]: first pair of each CTA, tiles of it that belong to CTAs before
   int* status;
 };
 
@@ -97,6 +108,8 @@ struct Shape {
   static constexpr int R = 2 * RH;          // rows, padded
   static constexpr int NS = pad16(QP * R);  // N of the score product
   static constexpr int WP = QP + 1;
+  static constexpr int MAX_STACK = RH <= 8 ? WP : RH <= 12 ? 3 : 2;  // registers of the epilogue
+  static constexpr int EPI_BOXES = MAX_STACK * RH <= 16 ? 3 : MAX_STACK * RH <= 24 ? 2 : 1;
 };
 
 KIMI_D bool elect_one() {
@@ -104,25 +117,58 @@ KIMI_D bool elect_one() {
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(e));
   return e != 0;
 }
-KIMI_D void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// Descriptors as (low, high) words: a step along a tile only moves the low word's address field.
+KIMI_D void mma_f8(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                   uint32_t accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "{\n .reg .pred p;\n .reg .b64 a, b;\n mov.b64 a, {%1, %2};\n mov.b64 b, {%3, %4};\n setp.ne.b32 p, %6, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %5, p;\n}\n" ::"r"(d),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+KIMI_D void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(
+                   tc::smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(tc::smem_u32(bar))
+               : "memory");
+}
+// Whether the phase of this parity is over; does not block.
+KIMI_D bool mbar_over(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(done)
+      : "r"(tc::smem_u32(bar)), "r"(parity & 1)
+      : "memory");
+  return done != 0;
+}
+// Programmatic dependent launch: let the next kernel of the stream start / wait for the one before.
+KIMI_D void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
+KIMI_D void pdl_wait() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
 // kind::f8f6f4 instruction descriptor: fp32 accumulator, A e4m3 (0), B e4m3 (0) or e5m2 (1).
 __host__ __device__ constexpr uint32_t idesc_f8(int m, int n, bool a_mn, bool b_e5m2) {
   return (1u << 4) | ((b_e5m2 ? 1u : 0u) << 10) | ((a_mn ? 1u : 0u) << 15) | ((uint32_t)(n >> 3) << 17) |
          ((uint32_t)(m >> 4) << 24);
 }
-KIMI_D void tmem_ld4(uint32_t addr, float* v) {
-  uint32_t r[4];
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];\n"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
+// N consecutive columns (a multiple of 4) of this warp's 32 lanes; complete after tmem_wait_ld.
+template <int N>
+KIMI_D void tmem_ldn(uint32_t addr, float* v) {
+  if constexpr (N >= 8) {
+    uint32_t r[8];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(addr));
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(r[i]);
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
+    if constexpr (N > 8) tmem_ldn<N - 8>(addr + 8, v + 8);
+  } else {
+    uint32_t r[4];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(r[i]);
+  }
 }
 // N columns of lanes 0-15 for each half of the warp: threads 16-31 get the columns SPLIT further on.
 template <int N, int SPLIT>
@@ -157,9 +203,15 @@ KIMI_D void tmem_st1(uint32_t addr, float v) {
 }
 KIMI_D void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
 KIMI_D void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
-KIMI_D void group_sync(int id) { asm volatile("bar.sync %0, 128;\n" ::"r"(id) : "memory"); }
+// The .aligned instructions of the compute groups want whole converged warps: each is behind a __syncwarp
+// where a lane-dependent branch comes before it.
+KIMI_D void group_sync(int id) {
+  __syncwarp();
+  asm volatile("bar.sync %0, 128;\n" ::"r"(id) : "memory");
+}
 KIMI_D bool group_any(int id, bool v) {
   uint32_t r;
+  __syncwarp();
   asm volatile(
       "{\n .reg .pred p, q;\n setp.ne.u32 p, %2, 0;\n bar.red.or.pred q, %1, 128, p;\n selp.u32 %0, 1, 0, q;\n}\n"
       : "=r"(r)
@@ -232,25 +284,130 @@ struct Walk {
   }
 };
 
+// Query parts, one warp per row, and (last block) the split of the tile list over the CTAs.
+template <typename T, int QP>
+__global__ void __launch_bounds__(256) attn_tc_prep_kernel(const __grid_constant__ TcParams p) {
+  __shared__ int swsum[8];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int pairs = p.a.batch * p.row_tiles, R = p.r_pad, NS = p.ns;
+  pdl_launch();
+  pdl_wait();
+  if (blockIdx.x == gridDim.x - 1) {
+    if (p.direct) return;
+    // Every thread counts the tiles of a run of pairs; a block scan places the runs in the list.
+    int64_t len, start;
+    const int run = (pairs + 255) / 256, v0 = min(tid * run, pairs), v1 = min(v0 + run, pairs);
+    int own = 0;
+    for (int v = v0; v < v1; ++v) own += pair_tiles(p, v, &len, &start);
+    int incl = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    if (lane == 31) swsum[warp] = incl;
+    __syncthreads();
+    int at = incl - own, total = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i < warp) at += swsum[i];
+      total += swsum[i];
+    }
+    const int per = max(p.min_tiles, (total + p.grid - 1) / p.grid);  // grid * per < 2^31: the host bounds the tiles
+    for (int v = v0; v < v1; ++v) {
+      const int n = run == 1 ? own : pair_tiles(p, v, &len, &start);
+      p.prefix[v] = at;
+      for (int c = (at + per - 1) / per; c * per < at + n; ++c) {  // CTAs that start inside this pair
+        p.first[2 * c] = v;
+        p.first[2 * c + 1] = c * per - at;
+      }
+      at += n;
+    }
+    if (tid == 0) {
+      p.prefix[pairs] = total;
+      p.prefix[pairs + 1] = per;
+    }
+    return;
+  }
+  const int row = blockIdx.x * 8 + warp;
+  if (row >= pairs * p.rows_tile) return;
+  const int v = row / p.rows_tile, r = row - v * p.rows_tile;
+  const int b = v / p.row_tiles, qr = (v - b * p.row_tiles) * p.rows_tile + r;
+  if (qr >= p.rows) return;
+  const int qi = qr / p.a.heads, h = qr - qi * p.a.heads;
+  const T* q = static_cast<const T*>(p.a.q) + b * p.a.q_b + qi * p.a.q_i + h * p.a.q_h;
+  const int octs = p.a.cache.width >> 3;
+  int4 x[kOcts];
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < kOcts; ++i) {
+    const int o = lane + 32 * i;
+    x[i] = make_int4(0, 0, 0, 0);
+    if (o < octs) {
+      if (p.q_vec) {
+        x[i] = __ldg(reinterpret_cast<const int4*>(q) + o);
+      } else {
+        Vec<T> e;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e.v[j] = q[o * 8 + j];
+        x[i] = *reinterpret_cast<const int4*>(e.v);
+      }
+    }
+    const uint32_t m = 0x7FFF7FFFu;
+    top = __vmaxu2(__vmaxu2(top, __vmaxu2(x[i].x & m, x[i].y & m)), __vmaxu2(x[i].z & m, x[i].w & m));
+  }
+  top = __reduce_max_sync(0xffffffffu, max(top & 0xFFFFu, top >> 16));
+  const unsigned short top16 = (unsigned short)top;
+  top = __float_as_uint(to_f<T>(*reinterpret_cast<const T*>(&top16)));
+  const bool bad = top >= 0x7F800000u;
+  const int k = bad ? 0 : min(126, 134 - (int)(top >> 23));  // the maximum to [128, 256)
+  const float f = pow2i(k);
+  uint8_t* image = p.q_parts + (int64_t)v * p.q_bytes;
+#pragma unroll
+  for (int i = 0; i < kOcts; ++i) {
+    const int o = lane + 32 * i;
+    if (o >= p.boxes * 16) break;
+    Vec<T> e;
+    *reinterpret_cast<int4*>(e.v) = x[i];
+    float y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = bad ? 0.f : e.f(j) * f;
+    uint8_t* at = image + (size_t)(o >> 4) * NS * 128 + (o & 1) * 8;
+#pragma unroll
+    for (int part = 0; part < QP; ++part) {
+      const int n = part * R + r;
+      uint32_t c[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        c[j] = to_codes2(y[2 * j], y[2 * j + 1]);
+        const float2 d = codes2(c[j]);
+        y[2 * j] = (y[2 * j] - d.x) * 32.f;
+        y[2 * j + 1] = (y[2 * j + 1] - d.y) * 32.f;
+      }
+      *reinterpret_cast<uint2*>(at + (n >> 3) * 1024 + (n & 7) * 128 + ((((o >> 1) & 7) ^ (n & 7)) << 4)) =
+          make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+    }
+  }
+  if (lane == 0) p.coef[v * R + r] = bad ? __uint_as_float(0x7FC00000u) : p.a.scale * kLog2e * pow2i(-k);
+}
+
 template <typename T, int RH, int QP>
 __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_constant__ TcParams p) {
   using S = Shape<RH, QP>;
   constexpr int R = S::R, HR = RH / 2;  // a thread of a compute group handles HR rows of one token
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* ring = smem_raw + ((1024u - (tc::smem_u32(smem_raw) & 1023u)) & 1023u);  // [slots][kBox]
-  uint8_t* sq = ring + (size_t)p.slots * kBox;                // [boxes][NS][128] query parts
-  uint8_t* sp = sq + (size_t)p.boxes * S::NS * 128;           // [2][p_bytes] weight parts
-  float4* sfac = reinterpret_cast<float4*>(sp + 2 * p.p_bytes);  // [R] normalisation of a row
+  uint8_t* ring = smem_raw + ((1024u - (tc::smem_u32(smem_raw) & 1023u)) & 1023u);  // [stages][group][kBox]
+  uint8_t* sq = ring + (size_t)p.stages * p.group * kBox;     // [boxes][NS][128] query parts
+  uint8_t* sp = sq + p.q_bytes;                               // [2][p_bytes] weight parts
+  float2* sfac = reinterpret_cast<float2*>(sp + 2 * p.p_bytes);  // [R] normalisation of a row
   float* sref = reinterpret_cast<float*>(sfac + R);           // [R] weight references
   float* sreft = sref + R;                                    // [R] sum references
-  float* scoef = sreft + R;                                   // [R] score factors
-  float* sdel = scoef + R;                                    // [R] change of a weight reference
+  float* sdel = sreft + R;                                    // [R] change of a weight reference
   float* smul = sdel + R;                                     // [R] factor of a sum
   float* sred = smul + R;                                     // [2 kinds][4 warps][R]
-  int* slim = reinterpret_cast<int*>(sred + 8 * R);           // [R] keys that a row sees
-  uint64_t* full = reinterpret_cast<uint64_t*>(slim + R);
-  uint64_t* empty = full + kMaxSlots;
-  uint64_t* s_full = empty + kMaxSlots;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sred + 8 * R);
+  uint64_t* empty = full + kMaxStages;
+  uint64_t* s_full = empty + kMaxStages;
   uint64_t* s_empty = s_full + 2;
   uint64_t* p_full = s_empty + 2;
   uint64_t* pv_done = p_full + 2;
@@ -258,7 +415,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
   uint64_t* drain = q_full + 1;
   uint32_t* tslot = reinterpret_cast<uint32_t*>(drain + 1);
   int* swalk = reinterpret_cast<int*>(tslot + 1);             // [3] first pair, skip, tiles
-  int* swsum = swalk + 3;                                     // [10] tiles counted by each warp
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int pairs = p.a.batch * p.row_tiles;
@@ -266,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 
   // ---- set-up: barriers, TMEM, this CTA's share of the tiles
   if (warp == 1) tc::tmem_alloc(tslot, p.tmem);
-  if (tid < p.slots) {
+  if (tid < p.stages) {
     tc::mbar_init(&full[tid], 1);
     tc::mbar_init(&empty[tid], 1);
   }
@@ -277,65 +433,30 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     tc::mbar_init(&pv_done[tid - 64], 1);
   }
   if (tid == 96) {
-    tc::mbar_init(q_full, 8);
+    tc::mbar_init(q_full, 1);
     tc::mbar_init(drain, 1);
     tc::tma_prefetch(&p.map);
-  }
-  {
-    // Every thread counts the tiles of a run of pairs; a block scan places the runs in the tile list.
-    int64_t len, start;
-    if (p.direct) {
-      if (tid == 0) {
-        swalk[0] = blockIdx.x;
-        swalk[1] = 0;
-        swalk[2] = pair_tiles(p, blockIdx.x, &len, &start);
-      }
-    } else {
-      const int run = (pairs + kThreads - 1) / kThreads, v0 = min(tid * run, pairs), v1 = min(v0 + run, pairs);
-      int own = 0;
-      for (int v = v0; v < v1; ++v) own += pair_tiles(p, v, &len, &start);
-      int incl = own;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += y;
-      }
-      if (lane == 31) swsum[warp] = incl;
-      if (tid == 0) {
-        swalk[0] = pairs;
-        swalk[1] = swalk[2] = 0;
-      }
-      __syncthreads();
-      int at = incl - own, total = 0;
-#pragma unroll
-      for (int i = 0; i < kThreads / 32; ++i) {
-        if (i < warp) at += swsum[i];
-        total += swsum[i];
-      }
-      const int per = max(p.min_tiles, (total + (int)gridDim.x - 1) / (int)gridDim.x);
-      const int mine = blockIdx.x * per;  // < 2^31: the host bounds the number of tiles
-      if (blockIdx.x == 0 || (mine >= at && mine < at + own)) {
-        for (int v = v0; v < v1; ++v) {
-          const int n = run == 1 ? own : pair_tiles(p, v, &len, &start);
-          if (blockIdx.x == 0) p.prefix[v] = at;
-          if (mine >= at && mine < at + n) {
-            swalk[0] = v;
-            swalk[1] = mine - at;
-            swalk[2] = min(per, total - mine);
-          }
-          at += n;
-        }
-      }
-      if (blockIdx.x == 0 && tid == 0) {
-        p.prefix[pairs] = total;
-        p.prefix[pairs + 1] = per;
-      }
-    }
   }
   // a context product may read weight parts that no row has: zeros
   for (int i = tid; i < 2 * p.p_bytes / 16; i += kThreads) reinterpret_cast<int4*>(sp)[i] = make_int4(0, 0, 0, 0);
   tc::fence_barrier_init();
   tc::fence_proxy_async();
+  pdl_launch();
+  pdl_wait();  // the query parts and the split are there
+  if (tid == 0) {
+    if (p.direct) {
+      int64_t len, start;
+      swalk[0] = blockIdx.x;
+      swalk[1] = 0;
+      swalk[2] = pair_tiles(p, blockIdx.x, &len, &start);
+    } else {
+      const int total = p.prefix[pairs], per = p.prefix[pairs + 1], mine = (int)blockIdx.x * per;
+      const bool any = mine < total;
+      swalk[0] = any ? p.first[2 * blockIdx.x] : pairs;
+      swalk[1] = any ? p.first[2 * blockIdx.x + 1] : 0;
+      swalk[2] = any ? min(per, total - mine) : 0;
+    }
+  }
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
@@ -348,24 +469,26 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 
   if (warp == 0) {
     // ---- loads
-    if (lane == 0) {
+    if (elect_one()) {
       bool ok = true;
-      uint32_t n = 0;  // boxes loaded so far
-      int slot = 0;
-      uint32_t ph = 1;  // parity of the last release of `slot` before this use
+      uint32_t n = 0;  // stages loaded so far
+      int st = 0;
+      uint32_t ph = 1;  // parity of the last release of stage `st` before this use
       while (ok && w.next(p, pairs)) {
         const int b = w.v / p.row_tiles;
         for (int t = w.t0; ok && t < w.t1; ++t) {
           const int y = p.t_first ? t * kTile : (int)(b * p.z_mul), z = p.t_first ? (int)(b * p.z_mul) : t * kTile;
-          for (int k = 0; k < p.boxes; ++k, ++n) {
-            if (n >= (uint32_t)p.slots && !tc::mbar_wait(&empty[slot], ph, p.status, tc::kTimeoutEmpty)) {
+          for (int k = 0; k < p.boxes; k += p.group, ++n) {
+            if (n >= (uint32_t)p.stages && !tc::mbar_wait(&empty[st], ph, p.status, tc::kTimeoutEmpty)) {
               ok = false;
               break;
             }
-            tc::mbar_arrive_expect_tx(&full[slot], kBox);
-            tc::tma_load_3d(ring + (size_t)slot * kBox, &p.map, &full[slot], k * 128, y, z);
-            if (++slot == p.slots) {
-              slot = 0;
+            const int nb = min(p.group, p.boxes - k);
+            tc::mbar_arrive_expect_tx(&full[st], nb * kBox);
+            uint8_t* dst = ring + (size_t)(st * p.group) * kBox;
+            for (int i = 0; i < nb; ++i) tc::tma_load_3d(dst + i * kBox, &p.map, &full[st], (k + i) * 128, y, z);
+            if (++st == p.stages) {
+              st = 0;
               ph ^= 1;
             }
           }
@@ -373,74 +496,107 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         ++w.v;
       }
       // copies in flight land before the CTA ends
-      for (uint32_t i = n > (uint32_t)p.slots ? n - p.slots : 0; i < n; ++i)
-        tc::mbar_wait_local(&full[i % p.slots], (i / p.slots) & 1, p.status, tc::kTimeoutDrain, tc::kDrainNs);
+      for (uint32_t i = n > (uint32_t)p.stages ? n - p.stages : 0; i < n; ++i)
+        tc::mbar_wait_local(&full[i % p.stages], (i / p.stages) & 1, p.status, tc::kTimeoutDrain, tc::kDrainNs);
     }
+    __syncwarp();
   } else if (warp == 1) {
-    // ---- MMAs: the whole warp walks, one elected thread issues.  Issued under elect.sync with descriptors
-    // that are sums of precomputed ones, an MMA costs what the tensor core takes (28 clocks for a score
-    // step of 48 columns, 40 for a context step); behind a plain lane test the issue alone took 90 to 170.
-    bool ok = true;
-    uint32_t n_tile = 0, seg = 0;  // tiles and segments so far
-    int s_slot = 0, o_slot = 0;    // next box of the score and of the context stream
-    uint32_t s_ph = 0;
-    const uint32_t id_s = idesc_f8(64, S::NS, false, false), id_o = idesc_f8(128, p.np, true, true);
-    const uint64_t ad_s = tc::smem_desc_sw128(tc::smem_u32(ring), 16, 1024);
-    const uint64_t ad_o = tc::smem_desc_sw128(tc::smem_u32(ring), 8192, 1024);
-    const uint64_t bd_q = tc::smem_desc_sw128(tc::smem_u32(sq), 16, 1024);
-    const uint64_t bd_p = tc::smem_desc_sw128(tc::smem_u32(sp), 16, 1024);
-    auto wait = [&](uint64_t* bar, uint32_t par, int code) {
-      ok = __all_sync(0xffffffffu, ok && tc::mbar_wait(bar, par & 1, p.status, code));
-      tc::tc_fence_after();
-      return ok;
-    };
-    auto scores = [&](uint32_t g, int k0, int k1) {  // boxes [k0, k1) of tile g's score product
-      const uint32_t buf = p.s_bufs == 2 ? g & 1 : 0, use = p.s_bufs == 2 ? g >> 1 : g;
-      if (k0 == 0 && use > 0 && !wait(&s_empty[buf], use - 1, tc::kTimeoutTmemEmpty)) return;
-      for (int k = k0; k < k1; ++k) {
-        if (!wait(&full[s_slot], s_ph, tc::kTimeoutFull)) return;
-        if (elect_one()) {
-          const uint64_t ad = ad_s + (uint64_t)(s_slot * (kBox >> 4)), bd = bd_q + (uint64_t)(k * S::NS * 8);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) mma_f8(tm_s + buf * S::NS, ad + 2 * j, bd + 2 * j, id_s, (k | j) != 0);
-          if (k == p.boxes - 1) tc::mma_commit(&s_full[buf]);
-        }
-        __syncwarp();
-        if (++s_slot == p.slots) {
-          s_slot = 0;
-          s_ph ^= 1;
-        }
-      }
-    };
-    while (ok && w.next(p, pairs)) {
-      if (!wait(q_full, seg, tc::kTimeoutTmemEmpty)) break;
-      scores(n_tile, 0, p.boxes);
-      for (int t = w.t0; ok && t < w.t1; ++t, ++n_tile) {
-        const bool more = t + 1 < w.t1;
-        if (more && p.ahead > 0) scores(n_tile + 1, 0, p.ahead);
-        const uint32_t pb = n_tile & 1;
-        if (!ok || !wait(&p_full[pb], n_tile >> 1, tc::kTimeoutTmemFull)) break;
-        for (int k = 0; k < p.boxes; ++k) {
-          if (elect_one()) {
-            const uint64_t ad = ad_o + (uint64_t)(o_slot * (kBox >> 4)), bd = bd_p + (uint64_t)(pb * (p.p_bytes >> 4));
-            const uint32_t d = tmem + (uint32_t)(k * p.np);
-            for (int run = 0; run < p.runs; ++run) {
-              const uint64_t br = bd + (uint64_t)((run >> 1) * p.np * 8 + (run & 1) * 4);
-              mma_f8(d, ad, br, id_o, (t > w.t0 || run > 0) ? 1u : 0u);
-              mma_f8(d, ad + (4096 >> 4), br + 2, id_o, 1u);
-            }
-            tc::mma_commit(&empty[o_slot]);
-            if (k == p.boxes - 1) tc::mma_commit(&pv_done[pb]);
-          }
-          __syncwarp();
-          if (++o_slot == p.slots) o_slot = 0;
-        }
-        if (more && p.ahead < p.boxes) scores(n_tile + 1, p.ahead, p.boxes);
-      }
-      ++seg;
-      ++w.v;
-    }
+    // ---- MMAs.  Issued under elect.sync with descriptors that are sums of precomputed words, an MMA costs
+    // what the tensor core takes (28 clocks for a score step of 48 columns, 40 for a context step); behind
+    // a plain lane test the issue alone took 90 to 170.
     if (elect_one()) {
+      // Two streams over the same tiles, scores and context, each taken as soon as its operands are there:
+      // a context product goes first (it frees its tile's part of the ring), else the next stage of scores.
+      int s_st = 0, o_st = 0, s_i = 0;  // ring stages of the streams; stage of the score tile
+      uint32_t s_ph = 0, s_n = 0, o_n = 0, s_seg = 0, polls = 0;  // tiles and segments so far
+      bool s_open = false;
+      const uint32_t id_s = idesc_f8(64, S::NS, false, false), id_o = idesc_f8(128, p.np, true, true);
+      const uint64_t ad_k = tc::smem_desc_sw128(tc::smem_u32(ring), 16, 1024);
+      const uint64_t ad_mn = tc::smem_desc_sw128(tc::smem_u32(ring), 8192, 1024);
+      const uint64_t bd_q = tc::smem_desc_sw128(tc::smem_u32(sq), 16, 1024);
+      const uint64_t bd_p = tc::smem_desc_sw128(tc::smem_u32(sp), 16, 1024);
+      const uint32_t k_hi = (uint32_t)(ad_k >> 32), mn_hi = (uint32_t)(ad_mn >> 32), q_hi = (uint32_t)(bd_q >> 32),
+                     p_hi = (uint32_t)(bd_p >> 32);
+      const uint32_t stage16 = (uint32_t)(p.group * (kBox >> 4));
+      Walk ws = w, wo = w;
+      bool s_have = ws.next(p, pairs), o_have = wo.next(p, pairs);
+      int s_t = ws.t0, o_t = wo.t0;
+      uint64_t since = 0;
+      while (o_have) {
+        const uint32_t pb = o_n & 1;
+        if (mbar_over(&p_full[pb], o_n >> 1)) {
+          tc::tc_fence_after();
+          const uint32_t pd = (uint32_t)bd_p + pb * (uint32_t)(p.p_bytes >> 4);
+          uint32_t d = tmem;
+          for (int i = 0; i < p.tile_stages; ++i) {
+            const int nb = min(p.group, p.boxes - i * p.group);
+            uint32_t a = (uint32_t)ad_mn + o_st * stage16;
+            for (int k = 0; k < nb; ++k, a += kBox >> 4, d += p.np) {
+              mma_f8(d, a, mn_hi, pd, p_hi, id_o, o_t > wo.t0 ? 1u : 0u);
+              mma_f8(d, a + (4096 >> 4), mn_hi, pd + 2, p_hi, id_o, 1u);
+              for (int run = 1; run < p.runs; ++run) {
+                const uint32_t pr = pd + (uint32_t)((run >> 1) * p.np * 8 + (run & 1) * 4);
+                mma_f8(d, a, mn_hi, pr, p_hi, id_o, 1u);
+                mma_f8(d, a + (4096 >> 4), mn_hi, pr + 2, p_hi, id_o, 1u);
+              }
+            }
+            tc::mma_commit(&empty[o_st]);
+            if (++o_st == p.stages) o_st = 0;
+          }
+          tc::mma_commit(&pv_done[pb]);
+          ++o_n;
+          if (++o_t == wo.t1) {
+            ++wo.v;
+            o_have = wo.next(p, pairs);
+            o_t = wo.t0;
+          }
+          polls = 0;
+          continue;
+        }
+        if (s_have) {
+          const uint32_t buf = p.s_bufs == 2 ? s_n & 1 : 0, use = p.s_bufs == 2 ? s_n >> 1 : s_n;
+          if (!s_open && (use == 0 || mbar_over(&s_empty[buf], use - 1)) && (s_t > ws.t0 || mbar_over(q_full, s_seg)))
+            s_open = true;
+          if (s_open && mbar_over(&full[s_st], s_ph)) {
+            tc::tc_fence_after();
+            const uint32_t d = tm_s + buf * S::NS;
+            const int k0 = s_i * p.group, nb = min(p.group, p.boxes - k0);
+            uint32_t a = (uint32_t)ad_k + s_st * stage16, q = (uint32_t)bd_q + k0 * (S::NS * 8);
+            for (int k = 0; k < nb; ++k, a += kBox >> 4, q += S::NS * 8) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) mma_f8(d, a + 2 * j, k_hi, q + 2 * j, q_hi, id_s, (s_i | k | j) != 0);
+            }
+            if (++s_st == p.stages) {
+              s_st = 0;
+              s_ph ^= 1;
+            }
+            if (++s_i == p.tile_stages) {
+              tc::mma_commit(&s_full[buf]);
+              s_i = 0;
+              s_open = false;
+              ++s_n;
+              if (++s_t == ws.t1) {
+                ++ws.v;
+                s_have = ws.next(p, pairs);
+                s_t = ws.t0;
+                ++s_seg;
+              }
+            }
+            polls = 0;
+            continue;
+          }
+        }
+        if ((++polls & 1023u) == 0) {  // bounded like every wait
+          if (tc::status_peek(p.status) != 0) break;
+          const uint64_t now = tc::globaltimer_ns();
+          if (polls == 1024) {
+            since = now;
+          } else if (now - since > tc::kWaitNs) {
+            atomicCAS(p.status, 0, (int)tc::kTimeoutTmemFull);
+            break;
+          }
+        }
+      }
       tc::mma_commit(drain);
       tc::mbar_wait_local(drain, 0, p.status, tc::kTimeoutDrain, tc::kDrainNs);
     }
@@ -448,7 +604,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
   } else {
     // ---- compute groups: rows [grp * RH, grp * RH + RH) of the pair.  The score tile has M = 64: its tokens
     // lie in lanes 0-15 of each warp's quadrant, and the halves of a warp take half of the rows each.
-    const int grp = (warp - 2) >> 2, quad = warp & 3, bar_id = 1 + grp, cw = warp - 2;
+    const int grp = (warp - 2) >> 2, quad = warp & 3, bar_id = 1 + grp;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     const int tok = quad * 16 + (lane & 15);
     const int r0 = grp * RH, rr = r0 + (lane >> 4) * HR;  // rows of the group and of this thread
@@ -468,95 +624,50 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     // groups' named barriers always meet and the kernel ends (its results are void, as the status says).
     bool ok = true;
     uint32_t n_tile = 0;
-    int slot = 0;  // first box of the tile
+    int stage = 0;  // first stage of the tile
     auto wait = [&](uint64_t* bar, uint32_t use, int code) {  // the warp is converged again behind it
       ok = ok && tc::mbar_wait(bar, use & 1, p.status, code);
       __syncwarp();
       tc::tc_fence_after();
     };
-    while (w.next(p, pairs)) {
+    auto load_q = [&](int v) {
+      tc::mbar_arrive_expect_tx(q_full, p.q_bytes);
+      bulk_load(sq, p.q_parts + (int64_t)v * p.q_bytes, p.q_bytes, q_full);
+    };
+    bool have = w.next(p, pairs);
+    if (have && warp == 2 && elect_one()) load_q(w.v);
+    __syncwarp();
+    uint32_t seg = 0;
+    while (have) {
       const int b = w.v / p.row_tiles, row0 = (w.v - b * p.row_tiles) * p.rows_tile;
       const int nrow = min(p.rows_tile, p.rows - row0);
-      // -- query rows into parts; one warp per row, the second read of a row comes from L1
-#pragma unroll 1
-      for (int r = cw; r < R; r += 8) {
-        const int qr = row0 + min(r, nrow - 1), qi = qr / p.a.heads, h = qr - qi * p.a.heads;
-        const T* q = static_cast<const T*>(p.a.q) + b * p.a.q_b + qi * p.a.q_i + h * p.a.q_h;
-        const int64_t seen = w.start + qi + 1;
-        if (lane == 0) {
-          slim[r] = seen < 0 ? 0 : (int)(seen < w.len ? seen : w.len);
-          sref[r] = sreft[r] = -INFINITY;
-          scoef[r] = 0.f;
-        }
-        if (r >= nrow) continue;
-        const int octs = width >> 3;
-        auto load = [&](int o) {
-          int4 x = make_int4(0, 0, 0, 0);
-          if (o < octs) {
-            if (p.q_vec) {
-              x = __ldg(reinterpret_cast<const int4*>(q) + o);
-            } else {
-              Vec<T> e;
+      Walk nx = w;
+      ++nx.v;
+      const bool more = nx.next(p, pairs);
+      float coef[HR], ref[HR], reft[HR], sum[HR];
 #pragma unroll
-              for (int j = 0; j < 8; ++j) e.v[j] = q[o * 8 + j];
-              x = *reinterpret_cast<const int4*>(e.v);
-            }
-          }
-          return x;
-        };
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < kOcts; ++i) {
-          const int4 x = load(lane + 32 * i);
-          const uint32_t m = 0x7FFF7FFFu;
-          top = __vmaxu2(__vmaxu2(top, __vmaxu2(x.x & m, x.y & m)), __vmaxu2(x.z & m, x.w & m));
-        }
-        top = __reduce_max_sync(0xffffffffu, max(top & 0xFFFFu, top >> 16));
-        const unsigned short top16 = (unsigned short)top;
-        top = __float_as_uint(to_f<T>(*reinterpret_cast<const T*>(&top16)));
-        const bool bad = top >= 0x7F800000u;
-        const int k = bad ? 0 : min(126, 134 - (int)(top >> 23));  // the maximum to [128, 256)
-        const float f = pow2i(k);
-#pragma unroll 1
-        for (int o = lane; o < p.boxes * 16; o += 32) {
-          Vec<T> e;
-          *reinterpret_cast<int4*>(e.v) = load(o);
-          float v[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = bad ? 0.f : e.f(j) * f;
-          uint8_t* at = sq + (size_t)(o >> 4) * S::NS * 128 + (o & 1) * 8;
-#pragma unroll
-          for (int part = 0; part < QP; ++part) {
-            const int n = part * R + r;
-            uint32_t c[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              c[j] = to_codes2(v[2 * j], v[2 * j + 1]);
-              const float2 d = codes2(c[j]);
-              v[2 * j] = (v[2 * j] - d.x) * 32.f;
-              v[2 * j + 1] = (v[2 * j + 1] - d.y) * 32.f;
-            }
-            *reinterpret_cast<uint2*>(at + (n >> 3) * 1024 + (n & 7) * 128 + ((((o >> 1) & 7) ^ (n & 7)) << 4)) =
-                make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
-          }
-        }
-        if (lane == 0) scoef[r] = bad ? __uint_as_float(0x7FC00000u) : p.a.scale * kLog2e * pow2i(-k);
+      for (int r = 0; r < HR; ++r) {
+        coef[r] = rr + r < nrow ? p.coef[w.v * R + rr + r] : 0.f;
+        ref[r] = reft[r] = -INFINITY;
+        sum[r] = 0.f;
       }
-      tc::fence_proxy_async();
-      tc::tc_fence_before();
-      __syncwarp();
-      asm volatile("bar.sync 3, 256;\n" ::: "memory");
-      if (lane == 0) tc::mbar_arrive(q_full);
-      const int lim0 = slim[0];  // rows come in the order of their positions
-      float sum[HR];
-#pragma unroll
-      for (int r = 0; r < HR; ++r) sum[r] = 0.f;
+      if (quad == 0 && lane < RH) sref[r0 + lane] = sreft[r0 + lane] = -INFINITY;
+      auto keys = [&](int r) {  // keys that row r sees; rows come in the order of their positions
+        const int64_t seen = w.start + 1 + (p.a.queries == 1 ? 0 : (row0 + min(r, nrow - 1)) / p.a.heads);
+        return seen < 0 ? 0 : (int)(seen < w.len ? seen : w.len);
+      };
+      const int lim0 = keys(0);
       const float* scales = p.a.cache.scales + b * p.a.cache.scale_b;
+      float st_next = w.t0 * kTile + tok < w.len ? scales[(w.t0 * kTile + tok) * p.a.cache.scale_t] : 0.f;
       for (int t = w.t0; t < w.t1; ++t, ++n_tile) {
         const int at = t * kTile + tok;
-        const float st = at < w.len ? scales[at * p.a.cache.scale_t] : 0.f;
+        const float st = st_next, lg = log2f(st);
+        if (t + 1 < w.t1) st_next = at + kTile < w.len ? scales[(at + kTile) * p.a.cache.scale_t] : 0.f;
         const uint32_t buf = p.s_bufs == 2 ? n_tile & 1 : 0, pb = n_tile & 1;
         wait(&s_full[buf], p.s_bufs == 2 ? n_tile >> 1 : n_tile, tc::kTimeoutTmemFull);
+        // this segment's score products are done: the next one's queries may come in
+        if (t + 1 == w.t1 && more && warp == 2 && elect_one()) load_q(nx.v);
+        __syncwarp();
         float s[HR];
         {
           float v[QP][HR];
@@ -564,40 +675,38 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
           for (int part = 0; part < QP; ++part)
             tmem_ld_halves<HR, HR>(tm_s + lanes + buf * S::NS + part * R + r0, v[part]);
           tmem_wait_ld();
+          tc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&s_empty[buf]);
 #pragma unroll
           for (int r = 0; r < HR; ++r) {
             float x = v[QP - 1][r];
 #pragma unroll
             for (int part = QP - 2; part >= 0; --part) x = fmaf(x, 0.03125f, v[part][r]);
-            s[r] = x * (scoef[rr + r] * st);
+            s[r] = x * (coef[r] * st);
           }
         }
-        tc::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&s_empty[buf]);
-        const float lg = log2f(st);
         uint32_t see = 0xFFFFFFFFu;
         if ((t + 1) * kTile > lim0) {  // a tile that some row does not see whole
           see = 0;
 #pragma unroll
-          for (int r = 0; r < HR; ++r) see |= (at < slim[rr + r] ? 1u : 0u) << r;
+          for (int r = 0; r < HR; ++r) see |= (at < keys(rr + r) ? 1u : 0u) << r;
           // slots past the length hold anything: their rows of the tile become zeros
           if ((int64_t)(t + 1) * kTile > w.len) {
             const int from = (int)(w.len - (int64_t)t * kTile), n = (kTile - from) * 8;
-            for (int k = 0, i = slot; k < p.boxes; ++k) {
-              uint8_t* box = ring + (size_t)i * kBox + from * 128;
+            for (int k = 0; k < p.boxes; ++k) {
+              const int st_k = (stage + k / p.group) % p.stages;
+              uint8_t* box = ring + (size_t)(st_k * p.group + k % p.group) * kBox + from * 128;
               for (int j = tid - 64; j < n; j += 256) reinterpret_cast<int4*>(box)[j] = make_int4(0, 0, 0, 0);
-              if (++i == p.slots) i = 0;
             }
           }
         }
-        slot += p.boxes;
-        if (slot >= p.slots) slot -= p.slots;
+        stage += p.tile_stages;
+        if (stage >= p.stages) stage -= p.stages;
         bool raise = false;
 #pragma unroll
         for (int r = 0; r < HR; ++r)
-          raise |= ((see >> r) & 1) && (s[r] + lg > sref[rr + r] + kTop || s[r] > sreft[rr + r] + kSumRoom);
-        __syncwarp();
+          raise |= ((see >> r) & 1) && (s[r] + lg > ref[r] + kTop || s[r] > reft[r] + kSumRoom);
         if (group_any(bar_id, raise)) {
           // some row outgrew a reference: new ones from the tile's maxima
 #pragma unroll
@@ -630,7 +739,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
           }
           group_sync(bar_id);
 #pragma unroll
-          for (int r = 0; r < HR; ++r) sum[r] *= smul[rr + r];
+          for (int r = 0; r < HR; ++r) {
+            sum[r] *= smul[rr + r];
+            ref[r] = sref[rr + r];
+            reft[r] = sreft[rr + r];
+          }
           if (t > w.t0) {  // the accumulators hold something
             bool waited = false;
 #pragma unroll 1
@@ -644,14 +757,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
               for (int g = 0; g < p.stack; ++g) {
                 const uint32_t c = tmem + lanes + (uint32_t)(g * R + r);
 #pragma unroll 1
-                for (int k = 0; k < p.boxes; k += 4) {
-                  float v[4];
+                for (int k = 0; k < p.boxes; k += 8) {
+                  float v[8];
 #pragma unroll
-                  for (int i = 0; i < 4; ++i)
+                  for (int i = 0; i < 8; ++i)
                     if (k + i < p.boxes) v[i] = tmem_ld1(c + (uint32_t)((k + i) * p.np));
                   tmem_wait_ld();
 #pragma unroll
-                  for (int i = 0; i < 4; ++i)
+                  for (int i = 0; i < 8; ++i)
                     if (k + i < p.boxes) tmem_st1(c + (uint32_t)((k + i) * p.np), v[i] * f.x * f.y);
                 }
               }
@@ -670,8 +783,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             const float x = s[r + e], ax = x + lg;
             const bool on = (see >> (r + e)) & 1;
             // a score of -inf weighs nothing, also against a reference of -inf
-            sum[r + e] += on && x != -INFINITY ? ex2(x - sreft[rr + r + e]) : 0.f;
-            v[e] = on && ax != -INFINITY ? ex2(ax - sref[rr + r + e]) : 0.f;
+            sum[r + e] += on && x != -INFINITY ? ex2(x - reft[r + e]) : 0.f;
+            v[e] = on && ax != -INFINITY ? ex2(ax - ref[r + e]) : 0.f;
           }
           // fp16 holds three parts; with four, the first comes off in fp32
           __half2 h;
@@ -711,45 +824,54 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         const float x = sred[r] + sred[R + r] + sred[2 * R + r] + sred[3 * R + r];
         // no key: the row is zeros; references are finite otherwise (or the row is NaN)
         const float2 f = x != 0.f ? pow2_pair(sref[r] - sreft[r]) : make_float2(0.f, 0.f);
-        sfac[r] = make_float4(f.x, f.y, x != 0.f ? 1.f / x : 0.f, 0.f);
+        sfac[r] = make_float2(f.x, x != 0.f ? f.y / x : 0.f);
         if (!whole && r < nrow) p.part_lse[part * p.rows_tile + r] = x != 0.f ? sreft[r] + log2f(x) : -INFINITY;
       }
       group_sync(bar_id);
       wait(&pv_done[(n_tile - 1) & 1], (n_tile - 1) >> 1, tc::kTimeoutTmemEmpty);
-      const int64_t first = whole ? (int64_t)b * p.rows + row0 + r0 : part * p.rows_tile + r0;
+      {
+        const int elt = whole ? (int)sizeof(T) : 4, have_rows = nrow - r0, l0 = quad * 32 + lane;
+        const int64_t row = whole ? (int64_t)b * p.rows + row0 + r0 : part * p.rows_tile + r0;
+        uint8_t* to = (whole ? static_cast<uint8_t*>(p.a.out) : reinterpret_cast<uint8_t*>(p.part_o)) +
+                      (row * width + l0) * elt;
+        const int step = width * elt;
 #pragma unroll 1
-      for (int k = 0; k < p.boxes; ++k) {
-        float v[RH];
+        for (int k = 0; k < p.boxes; k += S::EPI_BOXES) {
+          float v[S::EPI_BOXES][S::MAX_STACK][RH];
 #pragma unroll
-        for (int r = 0; r < RH; r += 4) tmem_ld4(tmem + lanes + (uint32_t)(k * p.np + r0 + r), v + r);
-        tmem_wait_ld();
-#pragma unroll 1
-        for (int g = 1; g < p.stack; ++g) {
-          float x[RH];
+          for (int i = 0; i < S::EPI_BOXES; ++i)
+            if (k + i < p.boxes) {
 #pragma unroll
-          for (int r = 0; r < RH; r += 4) tmem_ld4(tmem + lanes + (uint32_t)(k * p.np + g * R + r0 + r), x + r);
+              for (int g = 0; g < S::MAX_STACK; ++g)
+                if (g < p.stack) tmem_ldn<RH>(tmem + lanes + (uint32_t)((k + i) * p.np + g * R + r0), v[i][g]);
+            }
           tmem_wait_ld();
 #pragma unroll
-          for (int r = 0; r < RH; ++r) v[r] += x[r];
-        }
-        const int l = k * 128 + quad * 32 + lane;
-        if (l < width) {
-          const int64_t at = first * width + l;
+          for (int i = 0; i < S::EPI_BOXES; ++i, to += 128 * elt) {
+            const int rows = l0 + (k + i) * 128 < width ? have_rows : 0;
+            uint8_t* at = to;
 #pragma unroll
-          for (int r = 0; r < RH; ++r) {
-            if (r0 + r < nrow) {
-              const float4 f = sfac[r0 + r];
-              const float o = f.z == 0.f ? 0.f : v[r] * f.x * f.y * f.z;
-              if (whole) static_cast<T*>(p.a.out)[at + (int64_t)r * width] = from_f<T>(o);
-              else p.part_o[at + (int64_t)r * width] = o;
+            for (int r = 0; r < RH; ++r, at += step) {
+              const float2 f = sfac[r0 + r];
+              float x = v[i][0][r];
+#pragma unroll
+              for (int g = 1; g < S::MAX_STACK; ++g)
+                if (g < p.stack) x += v[i][g][r];
+              // no key: the accumulator may hold a stale column, the row is zeros
+              x = f.y == 0.f ? 0.f : x * f.x * f.y;
+              if (r < rows) {
+                if (whole) *reinterpret_cast<T*>(at) = from_f<T>(x);
+                else *reinterpret_cast<float*>(at) = x;
+              }
             }
           }
         }
       }
       tc::tc_fence_before();
-      __syncwarp();
-      asm volatile("bar.sync 3, 256;\n" ::: "memory");  // references and query rows are rewritten next
-      ++w.v;
+      group_sync(bar_id);  // references and sums of the group are rewritten next
+      w = nx;
+      have = more;
+      ++seg;
     }
     if (p.direct && swalk[2] == 0) {  // a pair without a key
       const int b = blockIdx.x / p.row_tiles, row0 = (blockIdx.x - b * p.row_tiles) * p.rows_tile;
@@ -757,8 +879,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       T* out = static_cast<T*>(p.a.out) + ((int64_t)b * p.rows + row0) * width;
       for (int64_t i = tid - 64; i < n; i += 256) out[i] = from_f<T>(0.f);
     }
+    // a query copy that nobody waited for (a wait failed before its turn) lands before the CTA ends
+    if (seg > 0 && warp == 2 && elect_one())
+      tc::mbar_wait_local(q_full, (seg - 1) & 1, p.status, tc::kTimeoutDrain, tc::kDrainNs);
+    __syncwarp();
   }
   tc::tc_fence_before();
+  __syncwarp();
   __syncthreads();
   if (warp == 1) {
     tc::tc_fence_after();
@@ -767,29 +894,61 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
   }
 }
 
-// Joins the CTAs of a pair: weights 2^(lse_c - max).  A pair inside one CTA is already written.
-template <typename T>
+// Joins the CTAs of a pair: weights 2^(lse_c - max), in the order of the CTAs.  A pair inside one CTA is
+// already written.  A block takes one row and 1,024 / SL columns; with many parts (a few long sequences) SL
+// groups of threads take every SL-th part each and are added up in shared memory.
+template <typename T, int SL>
 __global__ void __launch_bounds__(256) attn_tc_join_kernel(const __grid_constant__ TcParams p) {
+  constexpr int COLS = 256 / SL;  // threads along the columns, 4 columns each
+  __shared__ float4 sacc[SL > 1 ? SL : 1][COLS];
+  __shared__ float ssum[SL > 1 ? SL : 1];
   const int v = blockIdx.x / p.rows_tile, r = blockIdx.x - v * p.rows_tile;
   const int b = v / p.row_tiles, row0 = (v - b * p.row_tiles) * p.rows_tile, width = p.a.cache.width;
+  const int pairs = p.a.batch * p.row_tiles;
+  pdl_wait();
   if (row0 + r >= p.rows) return;
-  const int pairs = p.a.batch * p.row_tiles, per = p.prefix[pairs + 1];
-  const int at = p.prefix[v], n = p.prefix[v + 1] - at;
+  const int at = p.prefix[v], n = p.prefix[v + 1] - at, per = p.prefix[pairs + 1];
   const int c0 = n > 0 ? at / per : 0, c1 = n > 0 ? (at + n - 1) / per : -1;
   if (n > 0 && c0 == c1) return;
+  const int grp = threadIdx.x / COLS, l = (blockIdx.y * COLS + threadIdx.x % COLS) * 4;
+  const float* lse = p.part_lse + (int64_t)v * p.rows_tile + r;
   float m = -INFINITY;
-  for (int c = c0; c <= c1; ++c) m = fmaxf(m, p.part_lse[((int64_t)c + v) * p.rows_tile + r]);
+#pragma unroll 4
+  for (int c = c0; c <= c1; ++c) m = fmaxf(m, lse[(int64_t)c * p.rows_tile]);
   const float base = m == -INFINITY ? 0.f : m;
-  for (int l = blockIdx.y * 256 + threadIdx.x; l < width; l += gridDim.y * 256) {
-    float acc = 0.f, sum = 0.f;
-    for (int c = c0; c <= c1; ++c) {
-      const int64_t i = ((int64_t)c + v) * p.rows_tile + r;
-      const float f = exp2f(p.part_lse[i] - base);
-      sum += f;
-      acc += f * p.part_o[i * width + l];
-    }
-    static_cast<T*>(p.a.out)[((int64_t)b * p.rows + row0 + r) * width + l] = from_f<T>(sum != 0.f ? acc / sum : 0.f);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+  const float* po = p.part_o + ((int64_t)v * p.rows_tile + r) * width + (l < width ? l : 0);
+#pragma unroll 4
+  for (int c = c0 + grp; c <= c1; c += SL) {
+    const float f = exp2f(lse[(int64_t)c * p.rows_tile] - base);
+    const float4 x = *reinterpret_cast<const float4*>(po + (int64_t)c * p.rows_tile * width);
+    sum += f;
+    acc.x += f * x.x;
+    acc.y += f * x.y;
+    acc.z += f * x.z;
+    acc.w += f * x.w;
   }
+  if constexpr (SL > 1) {
+    sacc[grp][threadIdx.x % COLS] = acc;
+    if (threadIdx.x % COLS == 0) ssum[grp] = sum;
+    __syncthreads();
+    if (grp != 0) return;
+    for (int g = 1; g < SL; ++g) {
+      const float4 x = sacc[g][threadIdx.x];
+      acc.x += x.x;
+      acc.y += x.y;
+      acc.z += x.z;
+      acc.w += x.w;
+      sum += ssum[g];
+    }
+  }
+  if (l >= width) return;
+  const float inv = sum != 0.f ? 1.f / sum : 0.f;
+  T* out = static_cast<T*>(p.a.out) + ((int64_t)b * p.rows + row0 + r) * width + l;
+  const float o[4] = {acc.x, acc.y, acc.z, acc.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) out[i] = from_f<T>(inv == 0.f ? 0.f : o[i] * inv);
 }
 
 // Weight parts on N cost accumulator columns, parts along K cost a pass over the tile (36 + N / 5 clocks
@@ -799,34 +958,45 @@ bool fit(int boxes, Plan* pl) {
   using S = Shape<RH, QP>;
   bool found = false;
   int best = 0;
-  for (int stack = 1; stack <= S::WP; ++stack) {
+  for (int stack = 1; stack <= S::MAX_STACK; ++stack) {
     const int np = pad16(stack * S::R), runs = (S::WP + stack - 1) / stack, cols = boxes * np;
     const int bufs = cols + 2 * S::NS <= 512 ? 2 : cols + S::NS <= 512 ? 1 : 0;
     if (np > 256 || !bufs || (found && bufs < pl->s_bufs)) continue;
     const int cost = runs * (36 * 5 + np);
     if (found && cost >= best && bufs <= pl->s_bufs) continue;
     const int p_bytes = np * 128 * ((runs + 1) / 2);
-    const size_t fixed = (size_t)boxes * S::NS * 128 + 2 * p_bytes + (4 + 5 + 8 + 1) * S::R * 4 +
-                         (2 * kMaxSlots + 10) * 8 + 64 + 1024;  // + alignment
+    const size_t fixed = (size_t)boxes * S::NS * 128 + 2 * p_bytes + (2 + 4 + 8) * S::R * 4 +
+                         (2 * kMaxStages + 10) * 8 + 32 + 1024;  // + alignment
     if (fixed >= kSmemMax) continue;
-    int slots = (int)((kSmemMax - fixed) / kBox);
-    slots = slots < kMaxSlots ? slots : kMaxSlots;
-    if (slots < boxes + 2) continue;  // a tile and something to load meanwhile
+    // Stages as wide as the ring allows with a tile in it and more to load: a wide stage reads long pieces of
+    // each cached row together.
+    int tile_stages = 0, group = 0, stages = 0;
+    for (int g = kMaxGroup; g >= 1; --g) {
+      tile_stages = (boxes + g - 1) / g;
+      group = (boxes + tile_stages - 1) / tile_stages;
+      stages = (int)((kSmemMax - fixed) / (group * kBox));
+      stages = stages < kMaxStages ? stages : kMaxStages;
+      if (stages > tile_stages) break;
+    }
+    if (stages <= tile_stages) continue;
     found = true;
     best = cost;
     pl->rh = RH;
     pl->boxes = boxes;
-    pl->slots = slots;
+    pl->group = group;
+    pl->tile_stages = tile_stages;
+    pl->stages = stages;
     pl->s_bufs = bufs;
+    pl->ns = S::NS;
     pl->stack = stack;
     pl->runs = runs;
     pl->np = np;
     pl->p_bytes = p_bytes;
-    pl->ahead = slots - boxes < boxes ? slots - boxes : boxes;
+    pl->ahead = stages - tile_stages < tile_stages ? stages - tile_stages : tile_stages;
     uint32_t n = 32;
     while (n < (uint32_t)(cols + bufs * S::NS)) n *= 2;
     pl->tmem = n;
-    pl->smem = fixed + (size_t)slots * kBox;
+    pl->smem = fixed + (size_t)stages * group * kBox;
   }
   return found;
 }
@@ -846,7 +1016,6 @@ bool make_plan(const MlaCacheAttnArgs& a, Plan* pl) {
   KIMI_MLAC_FIT(8)
   KIMI_MLAC_FIT(12)
   KIMI_MLAC_FIT(16)
-  KIMI_MLAC_FIT(24)
 #undef KIMI_MLAC_FIT
   if (best.rh == 0) return false;
   *pl = best;
@@ -901,17 +1070,35 @@ int* status_ptr() {
   return g_status_addr[dev];
 }
 
+template <typename K>
+cudaError_t launch_dependent(K* kern, dim3 grid, int threads, size_t smem, cudaStream_t s, const TcParams& p) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, p);
+}
+
 template <typename T, int RH, int QP>
 cudaError_t launch(const TcParams& p, const Plan& pl, cudaStream_t s) {
   auto kern = attn_tc_kernel<T, RH, QP>;
   cudaError_t e = ensure_dynamic_smem(kern, (int)pl.smem);
   if (e != cudaSuccess) return e;
-  kern<<<pl.grid, kThreads, pl.smem, s>>>(p);
-  e = cudaGetLastError();
-  if (e != cudaSuccess || pl.direct) return e;
   const int pairs = p.a.batch * p.row_tiles;
-  attn_tc_join_kernel<T><<<dim3((unsigned)(pairs * p.rows_tile), (p.a.cache.width + 255) / 256), 256, 0, s>>>(p);
-  return cudaGetLastError();
+  e = launch_dependent(attn_tc_prep_kernel<T, QP>, dim3((pairs * p.rows_tile + 7) / 8 + 1), 256, 0, s, p);
+  if (e != cudaSuccess) return e;
+  if ((e = launch_dependent(kern, dim3(pl.grid), kThreads, pl.smem, s, p)) != cudaSuccess || pl.direct) return e;
+  const unsigned rows = (unsigned)(pairs * p.rows_tile);
+  const int width = p.a.cache.width;
+  if (pl.grid >= 8 * pairs)  // many parts of few pairs
+    return launch_dependent(attn_tc_join_kernel<T, 8>, dim3(rows, (width + 127) / 128), 256, 0, s, p);
+  return launch_dependent(attn_tc_join_kernel<T, 1>, dim3(rows, (width + 1023) / 1024), 256, 0, s, p);
 }
 
 template <typename T, int QP>
@@ -921,7 +1108,6 @@ cudaError_t launch_rh(const TcParams& p, const Plan& pl, cudaStream_t s) {
     case 8: return launch<T, 8, QP>(p, pl, s);
     case 12: return launch<T, 12, QP>(p, pl, s);
     case 16: return launch<T, 16, QP>(p, pl, s);
-    case 24: return launch<T, 24, QP>(p, pl, s);
     default: return cudaErrorInvalidValue;
   }
 }
@@ -938,11 +1124,26 @@ bool mla_attn_tc_supported(int dtype, const MlaCacheAttnArgs& a) {
   return plan_for(dtype, a, &pl);
 }
 
+// Layout of the workspace, in floats: query images, score factors, partial contexts and log-sums, the
+// tile list's prefix and the CTAs' first pairs.
+struct Work {
+  int64_t coef, part_o, part_lse, prefix, first, total;
+};
+static Work work_of(const MlaCacheAttnArgs& a, const Plan& pl) {
+  const int64_t pairs = (int64_t)a.batch * pl.row_tiles, units = pl.direct ? 0 : (pl.grid + pairs) * pl.rows_tile;
+  Work w;
+  w.coef = pairs * pl.boxes * pl.ns * 32;
+  w.part_o = w.coef + pairs * 2 * pl.rh;
+  w.part_lse = w.part_o + units * a.cache.width;
+  w.prefix = w.part_lse + units;
+  w.first = w.prefix + pairs + 2;
+  w.total = w.first + 2 * (int64_t)pl.grid;
+  return w;
+}
+
 int64_t mla_attn_tc_workspace(int dtype, const MlaCacheAttnArgs& a) {
   Plan pl;
-  if (!plan_for(dtype, a, &pl) || pl.direct) return 0;
-  const int64_t pairs = (int64_t)a.batch * pl.row_tiles;
-  return (pl.grid + pairs) * pl.rows_tile * (a.cache.width + 1) + pairs + 2;
+  return plan_for(dtype, a, &pl) ? work_of(a, pl).total : 0;
 }
 
 cudaError_t mla_attn_tc(int dtype, const MlaCacheAttnArgs& a, cudaStream_t s) {
@@ -955,17 +1156,23 @@ cudaError_t mla_attn_tc(int dtype, const MlaCacheAttnArgs& a, cudaStream_t s) {
   p.rows_tile = pl.rows_tile;
   p.row_tiles = pl.row_tiles;
   p.boxes = pl.boxes;
-  p.slots = pl.slots;
+  p.group = pl.group;
+  p.tile_stages = pl.tile_stages;
+  p.stages = pl.stages;
   p.s_bufs = pl.s_bufs;
   p.ahead = pl.ahead;
   p.stack = pl.stack;
   p.runs = pl.runs;
+  p.r_pad = 2 * pl.rh;
+  p.ns = pl.ns;
   p.np = pl.np;
   p.p_bytes = pl.p_bytes;
+  p.q_bytes = pl.boxes * pl.ns * 128;
+  p.grid = pl.grid;
   p.direct = pl.direct ? 1 : 0;
   p.min_tiles = 1;
-  p.q_vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.q_b % 8 == 0 && a.q_i % 8 == 0 && a.q_h % 8 == 0;
   p.tmem = pl.tmem;
+  p.q_vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.q_b % 8 == 0 && a.q_i % 8 == 0 && a.q_h % 8 == 0;
   const bool one = a.batch == 1 || a.cache.code_b == 0;  // every sequence reads the same rows
   p.z_mul = one ? 0 : 1;
   p.t_first = one || p.a.cache.code_t <= a.cache.code_b ? 1 : 0;
@@ -976,10 +1183,13 @@ cudaError_t mla_attn_tc(int dtype, const MlaCacheAttnArgs& a, cudaStream_t s) {
     bound = true;
   }
   if (!make_map(&p.map, p.a, p.t_first, one)) return cudaErrorInvalidValue;
-  const int64_t pairs = (int64_t)a.batch * pl.row_tiles, units = pl.direct ? 0 : (pl.grid + pairs) * pl.rows_tile;
-  p.part_o = a.part_acc;
-  p.part_lse = a.part_acc + units * a.cache.width;
-  p.prefix = reinterpret_cast<int*>(p.part_lse + units);
+  const Work wk = work_of(a, pl);
+  p.q_parts = reinterpret_cast<uint8_t*>(a.part_acc);
+  p.coef = a.part_acc + wk.coef;
+  p.part_o = a.part_acc + wk.part_o;
+  p.part_lse = a.part_acc + wk.part_lse;
+  p.prefix = reinterpret_cast<int*>(a.part_acc + wk.prefix);
+  p.first = reinterpret_cast<int*>(a.part_acc + wk.first);
   p.status = status_ptr();
   if (!p.status) return cudaErrorInvalidValue;
   return dtype == 1 ? launch_rh<__nv_bfloat16, 2>(p, pl, s) : launch_rh<__half, 3>(p, pl, s);

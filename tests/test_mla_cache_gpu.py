@@ -386,3 +386,21 @@ def test_refusals(cuda):
     assert empty.shape == (2, 0, 3, 64)
     ops.mla_cache_write(x.detach()[:, :0], codes, scales, n)
     assert not ops.mla_cache_attention(q.detach(), codes[:, :0], scales[:, :0], n).any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [(1, 3), (2, 8), (3, 8), (4, 8), (1, 24), (4, 12), (5, 10), (6, 12)],
+                         ids=lambda r: "x".join(map(str, r)))
+@pytest.mark.parametrize("width", [128, 640, 768, 1536])
+def test_attention_runs_of_tiles(cuda, width, rows, dtype):
+    """Batches large enough that a CTA walks several tiles and crosses from one sequence into the next, at every
+    number of query rows; lengths of every residue, empty sequences among them."""
+    from kimi_k3_b200 import ops
+    tq, h = rows
+    b, slots = 24, 1500
+    codes, scales = make_cache(b, slots, width, cuda)
+    q = queries(b, tq, h, width, dtype, cuda)
+    lens = torch.tensor([(i * 397) % (slots + 1) if i % 5 else (0, 1, 64, 65, slots)[i // 5] for i in range(b)], device=cuda)
+    out = ops.mla_cache_attention(q, codes, scales, lens, scale=0.6)
+    check_attention(out, q, codes, scales, lens, 0.6)
+    assert torch.equal(out, ops.mla_cache_attention(q, codes, scales, lens, scale=0.6))
