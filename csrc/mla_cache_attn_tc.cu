@@ -58,11 +58,16 @@ constexpr int kTile = 64;                  // tokens of a tile
 constexpr int kBox = kTile * 128;          // bytes of a box
 constexpr int kThreads = 320;
 constexpr int kMaxStages = 32;             // of the ring
+#ifndef FETCH
+#define FETCH 1
+#endif
 constexpr int kMaxGroup = 6;               // boxes of a stage
 constexpr int kSmemMax = 227 * 1024;
+constexpr int kMaxGrid = 256;              // CTAs of the attention kernel
 constexpr int kOcts = 8;                   // 8-element pieces of a query row per lane: widths up to 2,048
 constexpr float kTop = 15.f;               // a weight may reach 2^kTop
-constexpr float kRoom = 4.f;               // a new reference leaves this many bits
+constexpr float kRoom = 6.f;               // a new reference leaves this many bits
+constexpr float kNoRef = -3e38f;            // finite: a score of -inf weighs nothing against it
 constexpr float kSumRoom = 40.f;           // the sums' reference may lag by this many bits
 
 struct Plan {
@@ -88,7 +93,9 @@ struct Plan {
 struct TcParams {
   CUtensorMap map;
   MlaCacheAttnArgs a;
-  int rows, rows_tile, row_tiles, boxes, group, tile_stages, stages, s_bufs, ahead, direct, min_tiles, t_first, q_vec;
+  int rows, rows_tile, row_tiles, boxes, group, tile_stages, stages, s_bufs, ahead, direct, t_first, q_vec;
+  int wide;            // one copy per stage (L a multiple of 128), else one per box
+  int fetch;           // tiles ahead that are brought into L2
   int r_pad, stack, runs, ns, np, p_bytes, q_bytes, grid;
   uint32_t tmem;
   int64_t z_mul;       // 0 when every sequence reads the same cache rows
@@ -97,7 +104,6 @@ struct TcParams {
   float* part_o;       // [grid + pairs][rows_tile][L]
   float* part_lse;     // [grid + pairs][rows_tile]
   int* prefix;         // [pairs + 2]: first tile of each pair, total, tiles per CTA
-  int* first;          // [grid][2]: first pair of each CTA, tiles of it that belong to CTAs before
   int* status;
 };
 
@@ -130,6 +136,20 @@ KIMI_D void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar)
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(
                    tc::smem_u32(dst)),
                "l"(src), "r"(bytes), "r"(tc::smem_u32(bar))
+               : "memory");
+}
+// All boxes of a stage in one copy: tokens y.., 128-latent chunks c.. of sequence b; and the same into L2 only.
+KIMI_D void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int y, int c, int b) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];\n" ::"r"(tc::smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(y), "r"(c), "r"(b), "r"(tc::smem_u32(bar))
+      : "memory");
+}
+KIMI_D void tma_prefetch_4d(const CUtensorMap* map, int y, int c, int b) {
+  asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];\n" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(0), "r"(y), "r"(c), "r"(b)
                : "memory");
 }
 // Whether the phase of this parity is over; does not block.
@@ -225,6 +245,11 @@ KIMI_D float2 pow2_pair(float e) {
   const int n = (int)fminf(fmaxf(e, -250.f), 250.f), h = n / 2;
   return make_float2(pow2i(h), pow2i(n - h));
 }
+KIMI_D float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
 KIMI_D float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
@@ -284,51 +309,15 @@ struct Walk {
   }
 };
 
-// Query parts, one warp per row, and (last block) the split of the tile list over the CTAs.
+// Query parts, one warp per row.
 template <typename T, int QP>
 __global__ void __launch_bounds__(256) attn_tc_prep_kernel(const __grid_constant__ TcParams p) {
-  __shared__ int swsum[8];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int pairs = p.a.batch * p.row_tiles, R = p.r_pad, NS = p.ns;
-  pdl_launch();
   pdl_wait();
-  if (blockIdx.x == gridDim.x - 1) {
-    if (p.direct) return;
-    // Every thread counts the tiles of a run of pairs; a block scan places the runs in the list.
-    int64_t len, start;
-    const int run = (pairs + 255) / 256, v0 = min(tid * run, pairs), v1 = min(v0 + run, pairs);
-    int own = 0;
-    for (int v = v0; v < v1; ++v) own += pair_tiles(p, v, &len, &start);
-    int incl = own;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += y;
-    }
-    if (lane == 31) swsum[warp] = incl;
-    __syncthreads();
-    int at = incl - own, total = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (i < warp) at += swsum[i];
-      total += swsum[i];
-    }
-    const int per = max(p.min_tiles, (total + p.grid - 1) / p.grid);  // grid * per < 2^31: the host bounds the tiles
-    for (int v = v0; v < v1; ++v) {
-      const int n = run == 1 ? own : pair_tiles(p, v, &len, &start);
-      p.prefix[v] = at;
-      for (int c = (at + per - 1) / per; c * per < at + n; ++c) {  // CTAs that start inside this pair
-        p.first[2 * c] = v;
-        p.first[2 * c + 1] = c * per - at;
-      }
-      at += n;
-    }
-    if (tid == 0) {
-      p.prefix[pairs] = total;
-      p.prefix[pairs + 1] = per;
-    }
-    return;
-  }
+  // only now: the attention kernel reads cache and lengths without waiting for this one to end, so it may
+  // not start before everything ahead of this kernel is done
+  pdl_launch();
   const int row = blockIdx.x * 8 + warp;
   if (row >= pairs * p.rows_tile) return;
   const int v = row / p.rows_tile, r = row - v * p.rows_tile;
@@ -415,6 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
   uint64_t* drain = q_full + 1;
   uint32_t* tslot = reinterpret_cast<uint32_t*>(drain + 1);
   int* swalk = reinterpret_cast<int*>(tslot + 1);             // [3] first pair, skip, tiles
+  int* swsum = swalk + 3;                                     // [10] tiles counted by each warp
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int pairs = p.a.batch * p.row_tiles;
@@ -442,19 +432,54 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
   tc::fence_barrier_init();
   tc::fence_proxy_async();
   pdl_launch();
-  pdl_wait();  // the query parts and the split are there
-  if (tid == 0) {
-    if (p.direct) {
-      int64_t len, start;
+  if (p.direct) {
+    int64_t len, start;
+    if (tid == 0) {
       swalk[0] = blockIdx.x;
       swalk[1] = 0;
       swalk[2] = pair_tiles(p, blockIdx.x, &len, &start);
-    } else {
-      const int total = p.prefix[pairs], per = p.prefix[pairs + 1], mine = (int)blockIdx.x * per;
-      const bool any = mine < total;
-      swalk[0] = any ? p.first[2 * blockIdx.x] : pairs;
-      swalk[1] = any ? p.first[2 * blockIdx.x + 1] : 0;
-      swalk[2] = any ? min(per, total - mine) : 0;
+    }
+  } else {
+    // Every thread counts the tiles of a run of pairs; a block scan places the runs in the tile list.
+    int64_t len, start;
+    const int run = (pairs + kThreads - 1) / kThreads, v0 = min(tid * run, pairs), v1 = min(v0 + run, pairs);
+    int own = 0;
+    for (int v = v0; v < v1; ++v) own += pair_tiles(p, v, &len, &start);
+    __syncwarp();
+    int incl = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    if (lane == 31) swsum[warp] = incl;
+    if (tid == 0) {
+      swalk[0] = pairs;
+      swalk[1] = swalk[2] = 0;
+    }
+    __syncthreads();
+    int at = incl - own, total = 0;
+#pragma unroll
+    for (int i = 0; i < kThreads / 32; ++i) {
+      if (i < warp) at += swsum[i];
+      total += swsum[i];
+    }
+    const int per = (total + p.grid - 1) / p.grid, mine = (int)blockIdx.x * per;  // < 2^31: the host bounds the tiles
+    if (blockIdx.x == 0 || (mine >= at && mine < at + own)) {
+      for (int v = v0; v < v1; ++v) {
+        const int n = run == 1 ? own : pair_tiles(p, v, &len, &start);
+        if (blockIdx.x == 0) p.prefix[v] = at;
+        if (mine >= at && mine < at + n) {
+          swalk[0] = v;
+          swalk[1] = mine - at;
+          swalk[2] = min(per, total - mine);
+        }
+        at += n;
+      }
+    }
+    if (blockIdx.x == 0 && tid == 0) {
+      p.prefix[pairs] = total;
+      p.prefix[pairs + 1] = max(per, 1);
     }
   }
   tc::tc_fence_before();
@@ -475,18 +500,25 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       int st = 0;
       uint32_t ph = 1;  // parity of the last release of stage `st` before this use
       while (ok && w.next(p, pairs)) {
-        const int b = w.v / p.row_tiles;
+        const int zb = (int)((w.v / p.row_tiles) * p.z_mul);
         for (int t = w.t0; ok && t < w.t1; ++t) {
-          const int y = p.t_first ? t * kTile : (int)(b * p.z_mul), z = p.t_first ? (int)(b * p.z_mul) : t * kTile;
+          const bool fetch = p.fetch > 0 && t + p.fetch < w.t1;
           for (int k = 0; k < p.boxes; k += p.group, ++n) {
             if (n >= (uint32_t)p.stages && !tc::mbar_wait(&empty[st], ph, p.status, tc::kTimeoutEmpty)) {
               ok = false;
               break;
             }
-            const int nb = min(p.group, p.boxes - k);
-            tc::mbar_arrive_expect_tx(&full[st], nb * kBox);
             uint8_t* dst = ring + (size_t)(st * p.group) * kBox;
-            for (int i = 0; i < nb; ++i) tc::tma_load_3d(dst + i * kBox, &p.map, &full[st], (k + i) * 128, y, z);
+            if (p.wide) {  // chunks past the latent axis are filled with zeros and count
+              tc::mbar_arrive_expect_tx(&full[st], p.group * kBox);
+              tma_load_4d(dst, &p.map, &full[st], t * kTile, k, zb);
+              if (fetch) tma_prefetch_4d(&p.map, (t + p.fetch) * kTile, k, zb);
+            } else {
+              const int nb = min(p.group, p.boxes - k);
+              tc::mbar_arrive_expect_tx(&full[st], nb * kBox);
+              const int y = p.t_first ? t * kTile : zb, z = p.t_first ? zb : t * kTile;
+              for (int i = 0; i < nb; ++i) tc::tma_load_3d(dst + i * kBox, &p.map, &full[st], (k + i) * 128, y, z);
+            }
             if (++st == p.stages) {
               st = 0;
               ph ^= 1;
@@ -634,6 +666,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       tc::mbar_arrive_expect_tx(q_full, p.q_bytes);
       bulk_load(sq, p.q_parts + (int64_t)v * p.q_bytes, p.q_bytes, q_full);
     };
+    pdl_wait();  // the query parts are there
     bool have = w.next(p, pairs);
     if (have && warp == 2 && elect_one()) load_q(w.v);
     __syncwarp();
@@ -648,10 +681,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 #pragma unroll
       for (int r = 0; r < HR; ++r) {
         coef[r] = rr + r < nrow ? p.coef[w.v * R + rr + r] : 0.f;
-        ref[r] = reft[r] = -INFINITY;
+        ref[r] = reft[r] = kNoRef;
         sum[r] = 0.f;
       }
-      if (quad == 0 && lane < RH) sref[r0 + lane] = sreft[r0 + lane] = -INFINITY;
+      if (quad == 0 && lane < RH) sref[r0 + lane] = sreft[r0 + lane] = kNoRef;
       auto keys = [&](int r) {  // keys that row r sees; rows come in the order of their positions
         const int64_t seen = w.start + 1 + (p.a.queries == 1 ? 0 : (row0 + min(r, nrow - 1)) / p.a.heads);
         return seen < 0 ? 0 : (int)(seen < w.len ? seen : w.len);
@@ -661,7 +694,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       float st_next = w.t0 * kTile + tok < w.len ? scales[(w.t0 * kTile + tok) * p.a.cache.scale_t] : 0.f;
       for (int t = w.t0; t < w.t1; ++t, ++n_tile) {
         const int at = t * kTile + tok;
-        const float st = st_next, lg = log2f(st);
+        const float st = st_next;
+        const float lg = st < INFINITY ? lg2(st) : 0.f;  // a NaN stays in the scores of the rows that see it
         if (t + 1 < w.t1) st_next = at + kTile < w.len ? scales[(at + kTile) * p.a.cache.scale_t] : 0.f;
         const uint32_t buf = p.s_bufs == 2 ? n_tile & 1 : 0, pb = n_tile & 1;
         wait(&s_full[buf], p.s_bufs == 2 ? n_tile >> 1 : n_tile, tc::kTimeoutTmemFull);
@@ -686,11 +720,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             s[r] = x * (coef[r] * st);
           }
         }
-        uint32_t see = 0xFFFFFFFFu;
         if ((t + 1) * kTile > lim0) {  // a tile that some row does not see whole
-          see = 0;
 #pragma unroll
-          for (int r = 0; r < HR; ++r) see |= (at < keys(rr + r) ? 1u : 0u) << r;
+          for (int r = 0; r < HR; ++r)
+            if (at >= keys(rr + r)) s[r] = -INFINITY;
           // slots past the length hold anything: their rows of the tile become zeros
           if ((int64_t)(t + 1) * kTile > w.len) {
             const int from = (int)(w.len - (int64_t)t * kTile), n = (kTile - from) * 8;
@@ -703,16 +736,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         }
         stage += p.tile_stages;
         if (stage >= p.stages) stage -= p.stages;
+        float ev[HR], es[HR];  // log2 of the weights and of the sums' terms
         bool raise = false;
 #pragma unroll
-        for (int r = 0; r < HR; ++r)
-          raise |= ((see >> r) & 1) && (s[r] + lg > ref[r] + kTop || s[r] > reft[r] + kSumRoom);
+        for (int r = 0; r < HR; ++r) {
+          ev[r] = s[r] + lg - ref[r];
+          es[r] = s[r] - reft[r];
+          raise |= ev[r] > kTop || es[r] > kSumRoom;
+        }
         if (group_any(bar_id, raise)) {
           // some row outgrew a reference: new ones from the tile's maxima
 #pragma unroll
           for (int r = 0; r < HR; ++r) {
-            const bool on = (see >> r) & 1;
-            const float ma = half_max(on ? s[r] + lg : -INFINITY), ms = half_max(on ? s[r] : -INFINITY);
+            const float ma = half_max(s[r] + lg), ms = half_max(s[r]);
             if ((lane & 15) == 0) {
               sred[quad * R + rr + r] = ma;
               sred[(4 + quad) * R + rr + r] = ms;
@@ -743,6 +779,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             sum[r] *= smul[rr + r];
             ref[r] = sref[rr + r];
             reft[r] = sreft[rr + r];
+            ev[r] = s[r] + lg - ref[r];
+            es[r] = s[r] - reft[r];
           }
           if (t > w.t0) {  // the accumulators hold something
             bool waited = false;
@@ -752,7 +790,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
               if (del == 0.f) continue;  // uniform over the group
               if (!waited) wait(&pv_done[pb ^ 1], (n_tile - 1) >> 1, tc::kTimeoutTmemEmpty);
               waited = true;
-              const float2 f = del == -INFINITY ? make_float2(0.f, 0.f) : pow2_pair(del);
+              const float2 f = pow2_pair(del);
 #pragma unroll 1
               for (int g = 0; g < p.stack; ++g) {
                 const uint32_t c = tmem + lanes + (uint32_t)(g * R + r);
@@ -780,11 +818,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
           float v[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float x = s[r + e], ax = x + lg;
-            const bool on = (see >> (r + e)) & 1;
-            // a score of -inf weighs nothing, also against a reference of -inf
-            sum[r + e] += on && x != -INFINITY ? ex2(x - reft[r + e]) : 0.f;
-            v[e] = on && ax != -INFINITY ? ex2(ax - ref[r + e]) : 0.f;
+            sum[r + e] += ex2(es[r + e]);
+            v[e] = ex2(ev[r + e]);
           }
           // fp16 holds three parts; with four, the first comes off in fp32
           __half2 h;
@@ -901,7 +936,7 @@ template <typename T, int SL>
 __global__ void __launch_bounds__(256) attn_tc_join_kernel(const __grid_constant__ TcParams p) {
   constexpr int COLS = 256 / SL;  // threads along the columns, 4 columns each
   __shared__ float4 sacc[SL > 1 ? SL : 1][COLS];
-  __shared__ float ssum[SL > 1 ? SL : 1];
+  __shared__ float slse[SL > 1 ? kMaxGrid : 1], sstat[SL > 1 ? 2 * SL : 1];
   const int v = blockIdx.x / p.rows_tile, r = blockIdx.x - v * p.rows_tile;
   const int b = v / p.row_tiles, row0 = (v - b * p.row_tiles) * p.rows_tile, width = p.a.cache.width;
   const int pairs = p.a.batch * p.row_tiles;
@@ -910,45 +945,78 @@ __global__ void __launch_bounds__(256) attn_tc_join_kernel(const __grid_constant
   const int at = p.prefix[v], n = p.prefix[v + 1] - at, per = p.prefix[pairs + 1];
   const int c0 = n > 0 ? at / per : 0, c1 = n > 0 ? (at + n - 1) / per : -1;
   if (n > 0 && c0 == c1) return;
-  const int grp = threadIdx.x / COLS, l = (blockIdx.y * COLS + threadIdx.x % COLS) * 4;
+  const int col = threadIdx.x % COLS, grp = threadIdx.x / COLS, l = (blockIdx.y * COLS + col) * 4;
   const float* lse = p.part_lse + (int64_t)v * p.rows_tile + r;
-  float m = -INFINITY;
-#pragma unroll 4
-  for (int c = c0; c <= c1; ++c) m = fmaxf(m, lse[(int64_t)c * p.rows_tile]);
-  const float base = m == -INFINITY ? 0.f : m;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float sum = 0.f;
   const float* po = p.part_o + ((int64_t)v * p.rows_tile + r) * width + (l < width ? l : 0);
-#pragma unroll 4
-  for (int c = c0 + grp; c <= c1; c += SL) {
-    const float f = exp2f(lse[(int64_t)c * p.rows_tile] - base);
-    const float4 x = *reinterpret_cast<const float4*>(po + (int64_t)c * p.rows_tile * width);
-    sum += f;
-    acc.x += f * x.x;
-    acc.y += f * x.y;
-    acc.z += f * x.z;
-    acc.w += f * x.w;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float m = -INFINITY, sum = 0.f;
+  if constexpr (SL > 1) {  // all log-sums at once
+    const int parts = c1 - c0 + 1;  // <= kMaxGrid
+    for (int i = threadIdx.x; i < parts; i += 256) {
+      slse[i] = lse[(int64_t)(c0 + i) * p.rows_tile];
+      m = fmaxf(m, slse[i]);
+    }
+    m = warp_max(m);
+    if ((threadIdx.x & 31) == 0) sstat[threadIdx.x >> 5] = m;
+    __syncthreads();
+    m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, sstat[i]);
+  }
+  // four parts in flight; without the log-sums at hand the weights follow a running maximum
+  for (int c = c0 + grp; c <= c1; c += 4 * SL) {
+    float f[4];
+    float4 x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int ci = c + i * SL;
+      const bool on = ci <= c1;
+      f[i] = !on ? -INFINITY : SL > 1 ? slse[ci - c0] : lse[(int64_t)ci * p.rows_tile];
+      x[i] = on ? *reinterpret_cast<const float4*>(po + (int64_t)ci * p.rows_tile * width) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    if constexpr (SL == 1) {
+      const float to = fmaxf(fmaxf(m, fmaxf(f[0], f[1])), fmaxf(f[2], f[3]));
+      const float g = m == to || to == -INFINITY ? 1.f : exp2f(m - to);
+      m = to;
+      sum *= g;
+      acc.x *= g;
+      acc.y *= g;
+      acc.z *= g;
+      acc.w *= g;
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float e = exp2f(f[i] - base);  // 0 for a part that is not there
+      sum += e;
+      acc.x += e * x[i].x;
+      acc.y += e * x[i].y;
+      acc.z += e * x[i].z;
+      acc.w += e * x[i].w;
+    }
   }
   if constexpr (SL > 1) {
-    sacc[grp][threadIdx.x % COLS] = acc;
-    if (threadIdx.x % COLS == 0) ssum[grp] = sum;
+    sacc[grp][col] = acc;
+    if (col == 0) sstat[SL + grp] = sum;
     __syncthreads();
     if (grp != 0) return;
     for (int g = 1; g < SL; ++g) {
-      const float4 x = sacc[g][threadIdx.x];
+      const float4 x = sacc[g][col];
       acc.x += x.x;
       acc.y += x.y;
       acc.z += x.z;
       acc.w += x.w;
-      sum += ssum[g];
+      sum += sstat[SL + g];
     }
   }
   if (l >= width) return;
   const float inv = sum != 0.f ? 1.f / sum : 0.f;
   T* out = static_cast<T*>(p.a.out) + ((int64_t)b * p.rows + row0 + r) * width + l;
   const float o[4] = {acc.x, acc.y, acc.z, acc.w};
+  T t[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) out[i] = from_f<T>(inv == 0.f ? 0.f : o[i] * inv);
+  for (int i = 0; i < 4; ++i) t[i] = from_f<T>(inv == 0.f ? 0.f : o[i] * inv);
+  *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(t);
 }
 
 // Weight parts on N cost accumulator columns, parts along K cost a pass over the tile (36 + N / 5 clocks
@@ -966,7 +1034,7 @@ bool fit(int boxes, Plan* pl) {
     if (found && cost >= best && bufs <= pl->s_bufs) continue;
     const int p_bytes = np * 128 * ((runs + 1) / 2);
     const size_t fixed = (size_t)boxes * S::NS * 128 + 2 * p_bytes + (2 + 4 + 8) * S::R * 4 +
-                         (2 * kMaxStages + 10) * 8 + 32 + 1024;  // + alignment
+                         (2 * kMaxStages + 10) * 8 + 64 + 1024;  // + alignment
     if (fixed >= kSmemMax) continue;
     // Stages as wide as the ring allows with a tile in it and more to load: a wide stage reads long pieces of
     // each cached row together.
@@ -1023,7 +1091,7 @@ bool make_plan(const MlaCacheAttnArgs& a, Plan* pl) {
   pl->rows_tile = (rows + pl->row_tiles - 1) / pl->row_tiles;
   const int64_t pairs = (int64_t)a.batch * pl->row_tiles, tiles = (a.cache.slots + kTile - 1) / kTile;
   if (pairs > (1 << 20) || pairs * tiles > (1 << 30)) return false;
-  const int sms = device_sms();
+  const int sms = device_sms() < kMaxGrid ? device_sms() : kMaxGrid;
   pl->direct = tiles == 1;
   pl->grid = pl->direct ? (int)pairs : (int)(pairs * tiles < sms ? pairs * tiles : sms);
   return true;
@@ -1033,7 +1101,9 @@ bool plan_for(int dtype, const MlaCacheAttnArgs& a, Plan* pl) {
   return dtype == 1 ? make_plan<2>(a, pl) : make_plan<3>(a, pl);
 }
 
-bool make_map(CUtensorMap* m, const MlaCacheAttnArgs& a, bool t_first, bool one) {
+// wide: [B][L / 128][Tmax][128] as a view of the cache, boxes of `group` chunks x 64 tokens.  Else [B][Tmax][L]
+// with the smaller of the two outer strides first, boxes of 64 tokens x 128 latents (the last one partly zeros).
+bool make_map(CUtensorMap* m, const MlaCacheAttnArgs& a, bool wide, int group, bool t_first, bool one) {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
     cudaDriverEntryPointQueryResult q;
     void* ptr = nullptr;
@@ -1043,13 +1113,21 @@ bool make_map(CUtensorMap* m, const MlaCacheAttnArgs& a, bool t_first, bool one)
     return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
   }();
   if (!fn) return false;
-  const cuuint64_t nb = one ? 1 : a.batch, sb = one ? (cuuint64_t)a.cache.code_t * a.cache.slots : a.cache.code_b;
-  cuuint64_t dims[3] = {(cuuint64_t)a.cache.width, t_first ? (cuuint64_t)a.cache.slots : nb,
-                        t_first ? nb : (cuuint64_t)a.cache.slots};
-  cuuint64_t strides[2] = {t_first ? (cuuint64_t)a.cache.code_t : sb, t_first ? sb : (cuuint64_t)a.cache.code_t};
-  cuuint32_t box[3] = {128, t_first ? (cuuint32_t)kTile : 1u, t_first ? 1u : (cuuint32_t)kTile};
-  cuuint32_t estr[3] = {1, 1, 1};
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, a.cache.codes, dims, strides, box, estr,
+  const cuuint64_t slots = a.cache.slots, width = a.cache.width, ct = a.cache.code_t;
+  const cuuint64_t nb = one ? 1 : a.batch, cb = one ? ct * slots : a.cache.code_b;
+  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  cuuint64_t dims[4], strides[3];
+  cuuint32_t box[4];
+  if (wide) {
+    dims[0] = 128; dims[1] = slots; dims[2] = width / 128; dims[3] = nb;
+    strides[0] = ct; strides[1] = 128; strides[2] = cb;
+    box[0] = 128; box[1] = kTile; box[2] = group; box[3] = 1;
+  } else {
+    dims[0] = width; dims[1] = t_first ? slots : nb; dims[2] = t_first ? nb : slots;
+    strides[0] = t_first ? ct : cb; strides[1] = t_first ? cb : ct;
+    box[0] = 128; box[1] = t_first ? kTile : 1; box[2] = t_first ? 1 : kTile;
+  }
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, wide ? 4 : 3, a.cache.codes, dims, strides, box, ones,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -1091,7 +1169,7 @@ cudaError_t launch(const TcParams& p, const Plan& pl, cudaStream_t s) {
   cudaError_t e = ensure_dynamic_smem(kern, (int)pl.smem);
   if (e != cudaSuccess) return e;
   const int pairs = p.a.batch * p.row_tiles;
-  e = launch_dependent(attn_tc_prep_kernel<T, QP>, dim3((pairs * p.rows_tile + 7) / 8 + 1), 256, 0, s, p);
+  e = launch_dependent(attn_tc_prep_kernel<T, QP>, dim3((pairs * p.rows_tile + 7) / 8), 256, 0, s, p);
   if (e != cudaSuccess) return e;
   if ((e = launch_dependent(kern, dim3(pl.grid), kThreads, pl.smem, s, p)) != cudaSuccess || pl.direct) return e;
   const unsigned rows = (unsigned)(pairs * p.rows_tile);
@@ -1127,7 +1205,7 @@ bool mla_attn_tc_supported(int dtype, const MlaCacheAttnArgs& a) {
 // Layout of the workspace, in floats: query images, score factors, partial contexts and log-sums, the
 // tile list's prefix and the CTAs' first pairs.
 struct Work {
-  int64_t coef, part_o, part_lse, prefix, first, total;
+  int64_t coef, part_o, part_lse, prefix, total;
 };
 static Work work_of(const MlaCacheAttnArgs& a, const Plan& pl) {
   const int64_t pairs = (int64_t)a.batch * pl.row_tiles, units = pl.direct ? 0 : (pl.grid + pairs) * pl.rows_tile;
@@ -1136,8 +1214,7 @@ static Work work_of(const MlaCacheAttnArgs& a, const Plan& pl) {
   w.part_o = w.coef + pairs * 2 * pl.rh;
   w.part_lse = w.part_o + units * a.cache.width;
   w.prefix = w.part_lse + units;
-  w.first = w.prefix + pairs + 2;
-  w.total = w.first + 2 * (int64_t)pl.grid;
+  w.total = w.prefix + pairs + 2;
   return w;
 }
 
@@ -1169,8 +1246,8 @@ cudaError_t mla_attn_tc(int dtype, const MlaCacheAttnArgs& a, cudaStream_t s) {
   p.p_bytes = pl.p_bytes;
   p.q_bytes = pl.boxes * pl.ns * 128;
   p.grid = pl.grid;
+  p.fetch = FETCH;
   p.direct = pl.direct ? 1 : 0;
-  p.min_tiles = 1;
   p.tmem = pl.tmem;
   p.q_vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.q_b % 8 == 0 && a.q_i % 8 == 0 && a.q_h % 8 == 0;
   const bool one = a.batch == 1 || a.cache.code_b == 0;  // every sequence reads the same rows
@@ -1182,14 +1259,14 @@ cudaError_t mla_attn_tc(int dtype, const MlaCacheAttnArgs& a, cudaStream_t s) {
     (void)cudaFree(nullptr);
     bound = true;
   }
-  if (!make_map(&p.map, p.a, p.t_first, one)) return cudaErrorInvalidValue;
+  p.wide = a.cache.width % 128 == 0 ? 1 : 0;
+  if (!make_map(&p.map, p.a, p.wide, p.group, p.t_first, one)) return cudaErrorInvalidValue;
   const Work wk = work_of(a, pl);
   p.q_parts = reinterpret_cast<uint8_t*>(a.part_acc);
   p.coef = a.part_acc + wk.coef;
   p.part_o = a.part_acc + wk.part_o;
   p.part_lse = a.part_acc + wk.part_lse;
   p.prefix = reinterpret_cast<int*>(a.part_acc + wk.prefix);
-  p.first = reinterpret_cast<int*>(a.part_acc + wk.first);
   p.status = status_ptr();
   if (!p.status) return cudaErrorInvalidValue;
   return dtype == 1 ? launch_rh<__nv_bfloat16, 2>(p, pl, s) : launch_rh<__half, 3>(p, pl, s);
