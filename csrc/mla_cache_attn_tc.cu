@@ -58,9 +58,7 @@ constexpr int kTile = 64;                  // tokens of a tile
 constexpr int kBox = kTile * 128;          // bytes of a box
 constexpr int kThreads = 320;
 constexpr int kMaxStages = 32;             // of the ring
-#ifndef FETCH
-#define FETCH 1
-#endif
+constexpr int kFetch = 1;                  // tiles ahead that are brought into L2
 constexpr int kMaxGroup = 6;               // boxes of a stage
 constexpr int kSmemMax = 227 * 1024;
 constexpr int kMaxGrid = 256;              // CTAs of the attention kernel
@@ -103,7 +101,7 @@ struct TcParams {
   float* coef;         // [pairs][R] score factors
   float* part_o;       // [grid + pairs][rows_tile][L]
   float* part_lse;     // [grid + pairs][rows_tile]
-  int* prefix;         // [pairs + 2]: first tile of each pair, total, tiles per CTA
+  int* prefix;         // [pairs + 2]: first place of each pair, total, places per CTA
   int* status;
 };
 
@@ -287,9 +285,13 @@ KIMI_D int pair_tiles(const TcParams& p, int v, int64_t* len_out, int64_t* start
   return (int)((lim + kTile - 1) / kTile);
 }
 
-// This CTA's share of the tile list, walked pair by pair (every role walks it on its own).
+// The list of all pairs' tiles is cut into equal ranges, one per CTA.  Starting a pair costs a CTA about as
+// much as kStart tiles (an epilogue, an empty pipeline), so each pair with tiles has kStart places in front.
+constexpr int kStart = 2;
+
+// This CTA's share of the list, walked pair by pair (every role walks it on its own).
 struct Walk {
-  int v, skip, left;  // pair, tiles of it that belong to CTAs before, tiles of this CTA still to come
+  int v, skip, left;  // pair, tiles of it that belong to CTAs before, places from there to the range's end
   int t0, t1, tiles;  // the segment: tiles [t0, t1) of the pair's `tiles`
   int64_t len, start;
   KIMI_D bool next(const TcParams& p, int pairs) {
@@ -298,12 +300,11 @@ struct Walk {
       if (skip < tiles) {
         t0 = skip;
         t1 = min(tiles, skip + left);
-        left -= t1 - t0;
+        left -= t1 - t0 + kStart;  // the next pair's places in front
         skip = 0;
         return true;
       }
-      skip -= tiles;
-      ++v;
+      ++v;  // no tiles
     }
     return false;
   }
@@ -437,14 +438,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     if (tid == 0) {
       swalk[0] = blockIdx.x;
       swalk[1] = 0;
-      swalk[2] = pair_tiles(p, blockIdx.x, &len, &start);
+      swalk[2] = pair_tiles(p, blockIdx.x, &len, &start);  // all of it
     }
   } else {
     // Every thread counts the tiles of a run of pairs; a block scan places the runs in the tile list.
     int64_t len, start;
     const int run = (pairs + kThreads - 1) / kThreads, v0 = min(tid * run, pairs), v1 = min(v0 + run, pairs);
-    int own = 0;
-    for (int v = v0; v < v1; ++v) own += pair_tiles(p, v, &len, &start);
+    int own = 0, last = 0;
+    for (int v = v0; v < v1; ++v) {
+      last = pair_tiles(p, v, &len, &start);
+      own += last > 0 ? last + kStart : 0;
+    }
     __syncwarp();
     int incl = own;
 #pragma unroll
@@ -467,14 +471,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     const int per = (total + p.grid - 1) / p.grid, mine = (int)blockIdx.x * per;  // < 2^31: the host bounds the tiles
     if (blockIdx.x == 0 || (mine >= at && mine < at + own)) {
       for (int v = v0; v < v1; ++v) {
-        const int n = run == 1 ? own : pair_tiles(p, v, &len, &start);
+        const int n = run == 1 ? last : pair_tiles(p, v, &len, &start), places = n > 0 ? n + kStart : 0;
         if (blockIdx.x == 0) p.prefix[v] = at;
-        if (mine >= at && mine < at + n) {
+        if (mine >= at && mine < at + places) {
           swalk[0] = v;
-          swalk[1] = mine - at;
-          swalk[2] = min(per, total - mine);
+          swalk[1] = max(0, mine - at - kStart);
+          swalk[2] = mine + per - max(mine, at + kStart);
         }
-        at += n;
+        at += places;
       }
     }
     if (blockIdx.x == 0 && tid == 0) {
@@ -936,14 +940,15 @@ template <typename T, int SL>
 __global__ void __launch_bounds__(256) attn_tc_join_kernel(const __grid_constant__ TcParams p) {
   constexpr int COLS = 256 / SL;  // threads along the columns, 4 columns each
   __shared__ float4 sacc[SL > 1 ? SL : 1][COLS];
-  __shared__ float slse[SL > 1 ? kMaxGrid : 1], sstat[SL > 1 ? 2 * SL : 1];
+  __shared__ float slse[SL > 1 ? kMaxGrid : 1], sstat[SL > 1 ? 8 + SL : 1];
   const int v = blockIdx.x / p.rows_tile, r = blockIdx.x - v * p.rows_tile;
   const int b = v / p.row_tiles, row0 = (v - b * p.row_tiles) * p.rows_tile, width = p.a.cache.width;
   const int pairs = p.a.batch * p.row_tiles;
   pdl_wait();
   if (row0 + r >= p.rows) return;
-  const int at = p.prefix[v], n = p.prefix[v + 1] - at, per = p.prefix[pairs + 1];
-  const int c0 = n > 0 ? at / per : 0, c1 = n > 0 ? (at + n - 1) / per : -1;
+  const int at = p.prefix[v], places = p.prefix[v + 1] - at, per = p.prefix[pairs + 1];
+  const int n = places - kStart;  // tiles, if any
+  const int c0 = n > 0 ? (at + kStart) / per : 0, c1 = n > 0 ? (at + places - 1) / per : -1;
   if (n > 0 && c0 == c1) return;
   const int col = threadIdx.x % COLS, grp = threadIdx.x / COLS, l = (blockIdx.y * COLS + col) * 4;
   const float* lse = p.part_lse + (int64_t)v * p.rows_tile + r;
@@ -997,7 +1002,7 @@ __global__ void __launch_bounds__(256) attn_tc_join_kernel(const __grid_constant
   }
   if constexpr (SL > 1) {
     sacc[grp][col] = acc;
-    if (col == 0) sstat[SL + grp] = sum;
+    if (col == 0) sstat[8 + grp] = sum;
     __syncthreads();
     if (grp != 0) return;
     for (int g = 1; g < SL; ++g) {
@@ -1006,7 +1011,7 @@ __global__ void __launch_bounds__(256) attn_tc_join_kernel(const __grid_constant
       acc.y += x.y;
       acc.z += x.z;
       acc.w += x.w;
-      sum += sstat[SL + g];
+      sum += sstat[8 + g];
     }
   }
   if (l >= width) return;
@@ -1089,8 +1094,16 @@ bool make_plan(const MlaCacheAttnArgs& a, Plan* pl) {
   *pl = best;
   pl->row_tiles = (rows + 2 * best.rh - 1) / (2 * best.rh);
   pl->rows_tile = (rows + pl->row_tiles - 1) / pl->row_tiles;
+  if (pl->rows_tile <= 24 && best.rh > 12) {  // the rows of a tile pad less
+    Plan c;
+    if (fit<12, QP>(boxes, &c)) {
+      c.row_tiles = pl->row_tiles;
+      c.rows_tile = pl->rows_tile;
+      *pl = c;
+    }
+  }
   const int64_t pairs = (int64_t)a.batch * pl->row_tiles, tiles = (a.cache.slots + kTile - 1) / kTile;
-  if (pairs > (1 << 20) || pairs * tiles > (1 << 30)) return false;
+  if (pairs > (1 << 20) || pairs * tiles > (1 << 29)) return false;
   const int sms = device_sms() < kMaxGrid ? device_sms() : kMaxGrid;
   pl->direct = tiles == 1;
   pl->grid = pl->direct ? (int)pairs : (int)(pairs * tiles < sms ? pairs * tiles : sms);
@@ -1174,8 +1187,9 @@ cudaError_t launch(const TcParams& p, const Plan& pl, cudaStream_t s) {
   if ((e = launch_dependent(kern, dim3(pl.grid), kThreads, pl.smem, s, p)) != cudaSuccess || pl.direct) return e;
   const unsigned rows = (unsigned)(pairs * p.rows_tile);
   const int width = p.a.cache.width;
-  if (pl.grid >= 8 * pairs)  // many parts of few pairs
+  if (pl.grid >= 32 * pairs)  // many parts of few pairs
     return launch_dependent(attn_tc_join_kernel<T, 8>, dim3(rows, (width + 127) / 128), 256, 0, s, p);
+  if (pl.grid >= 6 * pairs) return launch_dependent(attn_tc_join_kernel<T, 2>, dim3(rows, (width + 511) / 512), 256, 0, s, p);
   return launch_dependent(attn_tc_join_kernel<T, 1>, dim3(rows, (width + 1023) / 1024), 256, 0, s, p);
 }
 
@@ -1246,7 +1260,7 @@ cudaError_t mla_attn_tc(int dtype, const MlaCacheAttnArgs& a, cudaStream_t s) {
   p.p_bytes = pl.p_bytes;
   p.q_bytes = pl.boxes * pl.ns * 128;
   p.grid = pl.grid;
-  p.fetch = FETCH;
+  p.fetch = kFetch;
   p.direct = pl.direct ? 1 : 0;
   p.tmem = pl.tmem;
   p.q_vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.q_b % 8 == 0 && a.q_i % 8 == 0 && a.q_h % 8 == 0;
