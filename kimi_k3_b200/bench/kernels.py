@@ -322,6 +322,22 @@ def bench_decode(args) -> list:
     tm = time_fn(lambda: C.mla_decode(qlat, latent, lengths), device=dev, warmup=args.warmup, repeats=args.repeats)
     rows.append(_emit({"case": "decode", "kernel": "mla_decode", "batch": b, "cache_tokens": t, "latent": l,
                        "heads": h, **tm.as_dict(), **roofline(tm.median_ms, bytes_moved=latent.numel() * 2)}))
+    # the same cache in 8 bits: the prompt's write, one token's write, the attention and the read-back
+    from .. import ops
+    codes = torch.zeros(b, t, l, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
+    scales = torch.zeros(b, t, device=dev)
+    zero = torch.zeros(b, dtype=torch.long, device=dev)
+    qh, token = qlat[:, None].bfloat16(), latent[:, :1].contiguous()
+    size = codes.numel()
+    for name, fn, moved in (
+            ("mla_cache_write_prompt", lambda: ops.mla_cache_write(latent, codes, scales, zero), 3 * size),
+            ("mla_cache_write_token", lambda: ops.mla_cache_write(token, codes, scales, zero), 3 * b * l),
+            ("mla_cache_attention", lambda: ops.mla_cache_attention(qh, codes, scales, lengths, scale=0.125), size),
+            ("mla_cache_read", lambda: ops.mla_cache_read(codes, scales, lengths), 3 * size)):
+        tc = time_fn(fn, device=dev, warmup=args.warmup, repeats=args.repeats)
+        rows.append(_emit({"case": "decode", "kernel": name, "batch": b, "cache_tokens": t, "latent": l, "heads": h,
+                           **tc.as_dict(), **roofline(tc.median_ms, bytes_moved=moved)}))
+    ops.mla_cache_check()
     q = torch.randn(b, h, 64, device=dev).bfloat16()
     g = -torch.rand(b, h, 64, device=dev)
     beta = torch.rand(b, h, device=dev)

@@ -534,6 +534,7 @@ def bench_decode(argv=None) -> list:
     p.add_argument("--vocab", type=int, default=50257)
     p.add_argument("--sample", action="store_true", help="top-k 50 / top-p 0.9 sampling instead of greedy")
     p.add_argument("--skip-eager", action="store_true")
+    p.add_argument("--cache-e4m3", action="store_true", help="also with the MLA latent cache in 8 bits")
     p.add_argument("--profile", action="store_true", help="print the per-kernel table of eager decode steps")
     args = p.parse_args(argv)
     dev = torch.device("cuda", 0)
@@ -573,6 +574,10 @@ def bench_decode(argv=None) -> list:
                                                                  max_name_column_width=60,
                                                                  max_shapes_column_width=80))
     run("cuda_graph_decoder", lambda: dec.generate(ids), args.new_tokens)
+    if args.cache_e4m3:
+        dec8 = GraphDecoder(model, max_length=args.prompt + args.new_tokens, generation_config=cfg,
+                            cache_dtype=torch.float8_e4m3fn)
+        run("cuda_graph_decoder_e4m3_cache", lambda: dec8.generate(ids), args.new_tokens)
     if not args.skip_eager:
         n = min(args.new_tokens, 32)
         ecfg = GenerationConfig(max_new_tokens=n, do_sample=args.sample, top_k=cfg.top_k, top_p=cfg.top_p, seed=0)

@@ -91,8 +91,14 @@ def cmd_infer(args) -> int:
     prompt = args.prompt
     if tok is None:
         prompt = [int(x) for x in prompt.split()]
+    cache_dtype = None
+    if args.cache_dtype == "e4m3":
+        import torch
+        if not args.graph:
+            raise SystemExit("--cache-dtype e4m3 needs the serving decoder (--graph)")
+        cache_dtype = torch.float8_e4m3fn
     out, ctx = run_distributed_generation(model_p, args.checkpoint, prompt, iy, tokenizer=tok,
-                                          precision=args.precision, use_graph=args.graph)
+                                          precision=args.precision, use_graph=args.graph, cache_dtype=cache_dtype)
     try:
         if ctx.is_global_zero:
             print(out.text if out.text is not None else out.sequences.tolist())
@@ -180,6 +186,8 @@ def build_parser() -> argparse.ArgumentParser:
             p.add_argument("--precision", choices=("model", "fp32", "bf16", "fp16"), default="model")
             p.add_argument("--graph", action="store_true",
                            help="serve the decode loop from one captured CUDA graph per token")
+            p.add_argument("--cache-dtype", choices=("model", "e4m3"), default="model",
+                           help="hold the MLA latent cache in the compute dtype or, with --graph, in 8 bits")
     sub.add_parser("smoke")
     pp = sub.add_parser("profiles")
     pp.add_argument("--output", default="configs/kimi_full_pipeline")

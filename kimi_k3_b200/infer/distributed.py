@@ -55,10 +55,11 @@ def graph_capturable(model: nn.Module) -> bool:
 
 
 def run_distributed_generation(model_config_path, checkpoint_path, prompt, inference_yaml, *, tokenizer=None,
-                               precision: str = "model", use_graph: bool = False, max_length: int | None = None):
+                               precision: str = "model", use_graph: bool = False, max_length: int | None = None,
+                               cache_dtype: torch.dtype | None = None):
     """Initialise the mesh from ``inference_yaml.distributed``, load, shard, generate.
 
-    Returns ``(output, context)``; the caller reports on ``context.is_global_zero`` and closes
+    ``cache_dtype`` is the serving decoder's (``use_graph``).  Returns ``(output, context)``; the caller reports on ``context.is_global_zero`` and closes
     the context."""
     from ..parallel.environment import setup_distributed
     from .config import ModelLoadConfig
@@ -76,7 +77,8 @@ def run_distributed_generation(model_config_path, checkpoint_path, prompt, infer
         from .graph_decode import GraphDecoder
         ids = encode_prompt(prompt, tokenizer=tokenizer, add_bos_token=gen.add_bos_token)
         ml = max_length or int(ids.shape[1]) + gen.max_new_tokens
-        dec = GraphDecoder(model, max_length=ml, generation_config=gen, use_graph=graph_capturable(model))
+        dec = GraphDecoder(model, max_length=ml, generation_config=gen, use_graph=graph_capturable(model),
+                           cache_dtype=cache_dtype)
         out = dec.generate(ids)
         dec.release()
     else:

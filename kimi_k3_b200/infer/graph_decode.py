@@ -8,7 +8,8 @@ and the same prefill, then
 * moves the prefill cache into serving buffers sized for ``max_length`` tokens: the KDA
   recurrent states and conv histories are advanced IN PLACE by the decode kernels
   (``KDAState(inplace=True)``), the MLA latents live in a :class:`StaticMLACache`
-  ``[B, max_length, L]`` that appends one row per step in place;
+  ``[B, max_length, L]`` that appends one row per step in place, or with ``cache_dtype=
+  torch.float8_e4m3fn`` in a :class:`QuantizedMLACache` of half its bytes;
 * captures one decode step -- embedding, every layer, LM head, the fused sampling kernel
   (repetition-penalty bitmap, temperature, top-k, top-p, Philox draw keyed by a device
   counter), EOS bookkeeping and the write of the token into a device output buffer -- in a
@@ -30,7 +31,7 @@ import torch.nn as nn
 
 from ..models.backbone import HybridBackboneCache, HybridLayerCache
 from ..models.kda import KDAState
-from ..models.mla import MLACache, StaticMLACache
+from ..models.mla import MLACache, QuantizedMLACache, StaticMLACache
 from ..models.primitives import ShortConvState
 from ..runtime import sync_free
 from .session import cache_summary
@@ -69,7 +70,7 @@ def serving_copy(model: nn.Module, dtype: torch.dtype, *, inplace: bool = False)
     return m.eval()
 
 
-def _static_layer(lc: HybridLayerCache, max_length: int) -> HybridLayerCache:
+def _static_layer(lc: HybridLayerCache, max_length: int, cache_dtype: torch.dtype | None = None) -> HybridLayerCache:
     s = lc.state
     if isinstance(s, KDAState):
         return HybridLayerCache("kda", KDAState(s.recurrent_state.float().clone(),
@@ -78,7 +79,8 @@ def _static_layer(lc: HybridLayerCache, max_length: int) -> HybridLayerCache:
                                                 ShortConvState(s.v_conv_state.buffer.clone()),
                                                 s.sequence_offset.clone(), inplace=True))
     if isinstance(s, MLACache):
-        return HybridLayerCache("gated_mla", StaticMLACache.from_cache(s, max_length))
+        kind = StaticMLACache if cache_dtype is None else QuantizedMLACache
+        return HybridLayerCache("gated_mla", kind.from_cache(s, max_length))
     raise TypeError(f"unsupported layer cache {type(s).__name__}")
 
 
@@ -92,6 +94,9 @@ def _load_static_layer(static: HybridLayerCache, lc: HybridLayerCache) -> None:
                          (s.v_conv_state, src.v_conv_state)):
             dst.buffer.copy_(new.buffer)
         s.sequence_offset.copy_(src.sequence_offset)
+        return
+    if isinstance(s, QuantizedMLACache):
+        s.load(src)
         return
     t = src.latent_kv.shape[1]
     if t > s.latent_kv.shape[1]:
@@ -111,6 +116,8 @@ def _state_tensors(cache: HybridBackboneCache) -> list:
                     s.sequence_offset]
         else:
             out += [s.latent_kv, s.sequence_offset]
+            if isinstance(s, QuantizedMLACache):
+                out.append(s.scales)
     return out
 
 
@@ -121,11 +128,15 @@ class GraphDecoder:
     ``autocast_dtype`` (bf16 by default on CUDA, None to disable) is the compute dtype of the
     prefill and of every decode step; with it the decoder serves from :func:`serving_copy` of the
     model (projection matrices stored in that dtype; ``copy_model=False`` converts the model itself
-    instead of a copy, for a model loaded only to serve)."""
+    instead of a copy, for a model loaded only to serve).  ``cache_dtype=torch.float8_e4m3fn`` holds the
+    MLA latents in 8 bits (None: in the dtype of the prefill's)."""
 
     def __init__(self, model, *, max_length: int, generation_config: GenerationConfig | None = None,
                  use_graph: bool | None = None, autocast_dtype: torch.dtype | None = torch.bfloat16,
-                 copy_model: bool = True):
+                 copy_model: bool = True, cache_dtype: torch.dtype | None = None):
+        if cache_dtype not in (None, torch.float8_e4m3fn):
+            raise ValueError(f"cache_dtype must be None or torch.float8_e4m3fn, got {cache_dtype}")
+        self.cache_dtype = cache_dtype
         self.max_length = int(max_length)
         self.cfg = generation_config or GenerationConfig()
         dev = next(model.parameters()).device
@@ -229,7 +240,7 @@ class GraphDecoder:
             else:
                 self.release()
                 self._key = key
-                self.cache = HybridBackboneCache(tuple(_static_layer(lc, self.max_length)
+                self.cache = HybridBackboneCache(tuple(_static_layer(lc, self.max_length, self.cache_dtype)
                                                        for lc in pre.cache.layer_caches), pre.cache.sequence_length)
                 self.tok = torch.zeros(b, 1, dtype=torch.long, device=dev)
                 self.out = torch.zeros(b, self.max_length, dtype=torch.long, device=dev)
@@ -278,6 +289,9 @@ class GraphDecoder:
                     reason = "eos"
             sync()
             decode_s = time.perf_counter() - t1
+            if self.cache_dtype is not None and dev.type == "cuda":
+                from .. import ops
+                ops.mla_cache_check()
         finally:
             if was_training:
                 model.train()
@@ -318,11 +332,12 @@ class GraphDecoder:
 
 def graph_generate(model, input_ids, *, max_length: int | None = None,
                    generation_config: GenerationConfig | None = None, attention_mask=None,
-                   use_graph: bool | None = None, prefill_kwargs: dict | None = None) -> GenerationOutput:
+                   use_graph: bool | None = None, prefill_kwargs: dict | None = None,
+                   cache_dtype: torch.dtype | None = None) -> GenerationOutput:
     """One-call form of :class:`GraphDecoder` (``max_length`` defaults to prompt + new tokens)."""
     cfg = generation_config or GenerationConfig()
     ml = max_length if max_length is not None else int(input_ids.shape[1]) + cfg.max_new_tokens
-    return GraphDecoder(model, max_length=ml, generation_config=cfg, use_graph=use_graph).generate(
+    return GraphDecoder(model, max_length=ml, generation_config=cfg, use_graph=use_graph, cache_dtype=cache_dtype).generate(
         input_ids, attention_mask, prefill_kwargs=prefill_kwargs)
 
 

@@ -13,7 +13,8 @@ Differences by design:
     (per-row key lengths instead of a materialised ``[B,Tq,Tk]`` mask);
   * the reference re-expands K/V from the whole latent cache every decode step;
     :func:`absorbed_latent_decode` folds ``W_uk`` into the query and ``W_uv`` into
-    the output so decode reads only the ``[T,L]`` latent cache.
+    the output so decode reads only the ``[T,L]`` latent cache;
+  * :class:`QuantizedMLACache` holds that cache in 8 bits (no counterpart in the reference).
 """
 from __future__ import annotations
 
@@ -227,6 +228,138 @@ class StaticMLACache(MLACache):
         return self
 
 
+# --------------------------------------------------------------------------- 8-bit cache
+E4M3 = torch.float8_e4m3fn
+E4M3_MAX = 448.0
+
+
+def quantize_latents(latent: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """``[...,L]`` -> float8_e4m3fn codes ``[...,L]`` and fp32 scales ``[...]``, value = code * scale.
+
+    A row's scale is the least power of two 2^k, k >= -126, with max |x| <= 448 * 2^k: the division is
+    exact and the values are exact in bf16.  A row holding a NaN or an infinity gets scale NaN, codes 0."""
+    x = latent.float()
+    top = x.abs().amax(dim=-1)
+    mantissa, exponent = torch.frexp(top)  # top = mantissa * 2^exponent, mantissa in [0.5, 1); 448 = 0.875 * 2^9
+    k = torch.where(mantissa <= 0.875, exponent - 9, exponent - 8)
+    k = torch.where(top == 0, torch.full_like(k, -126), k).clamp(min=-126)
+    scale = torch.ldexp(torch.ones_like(top), k)
+    bad = ~torch.isfinite(top)
+    codes = torch.where(bad[..., None], torch.zeros_like(x), x / scale[..., None]).to(E4M3)
+    return codes, torch.where(bad, torch.full_like(scale, math.nan), scale)
+
+
+def dequantize_latents(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    return (codes.float() * scales[..., None]).to(dtype)
+
+
+@dataclass(init=False)
+class QuantizedMLACache(StaticMLACache):
+    """A serving cache in 8 bits: e4m3 codes ``[B,Tmax,L]`` (``latent_kv``) and one fp32 scale per token
+    (``scales`` ``[B,Tmax]``); half the bytes of a bf16 :class:`StaticMLACache` and the same in-place
+    contract (valid rows are the prefix ``[0, sequence_offset[b])``, no host synchronisation).
+
+    Unlike the 16-bit cache it takes several tokens per row and call (``attention_mask`` ``[B,T]``,
+    right-padded, counts each row's), for prompt pieces and drafted tokens; with one token per call a row
+    that has reached ``Tmax`` keeps overwriting its last slot, with several the overhanging ones are
+    dropped.  On CUDA the hand-written kernels of ``ops.mla_cache_*`` run, elsewhere their definition."""
+
+    scales: torch.Tensor = None
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, sequence_offset: torch.Tensor):
+        if codes.dtype != E4M3 or scales.dtype != torch.float32 or tuple(scales.shape) != tuple(codes.shape[:2]):
+            raise ValueError("a quantized MLA cache takes float8_e4m3fn codes [B,T,L] and float32 scales [B,T]")
+        super().__init__(codes, sequence_offset)
+        self.scales = scales
+
+    @classmethod
+    def zeros(cls, batch_size: int, max_length: int, latent_dim: int, *, device=None) -> "QuantizedMLACache":
+        if batch_size <= 0 or max_length <= 0 or latent_dim <= 0:
+            raise ValueError("batch_size, max_length and latent_dim must be > 0")
+        codes = torch.zeros(batch_size, max_length, latent_dim, dtype=torch.uint8, device=device).view(E4M3)
+        return cls(codes, torch.zeros(batch_size, max_length, device=device),
+                   torch.zeros(batch_size, dtype=torch.long, device=device))
+
+    @classmethod
+    def from_cache(cls, cache: MLACache, max_length: int) -> "QuantizedMLACache":
+        b, t, l = cache.latent_kv.shape
+        if max_length < t:
+            raise ValueError(f"max_length {max_length} is shorter than the prefilled cache ({t})")
+        return cls.zeros(b, max_length, l, device=cache.latent_kv.device).load(cache)
+
+    def load(self, cache: MLACache) -> "QuantizedMLACache":
+        """Refill in place from a prefill cache (right-padded rows of ``sequence_offset`` tokens)."""
+        if cache.latent_kv.shape[1] > self.latent_kv.shape[1]:
+            raise ValueError(f"prompt of {cache.latent_kv.shape[1]} tokens exceeds the serving cache "
+                             f"({self.latent_kv.shape[1]})")
+        self.sequence_offset.zero_()
+        self._write(cache.latent_kv, self.sequence_offset, cache.sequence_offset)
+        self.sequence_offset.copy_(cache.sequence_offset)
+        return self
+
+    def _write(self, latent, offsets, counts=None) -> None:
+        if _ops.use_kernels(latent):
+            _ops.mla_cache_write(latent, self.latent_kv, self.scales, offsets, counts)
+            return
+        codes, scales = quantize_latents(latent)
+        step = torch.arange(latent.shape[1], device=latent.device)
+        slot = offsets[:, None] + step
+        keep = (slot >= 0) & (slot < self.latent_kv.shape[1])
+        if counts is not None:
+            keep = keep & (step < counts[:, None])
+        row, col = keep.nonzero(as_tuple=True)
+        self.latent_kv.view(torch.uint8)[row, slot[row, col]] = codes.view(torch.uint8)[row, col]
+        self.scales[row, slot[row, col]] = scales[row, col]
+
+    def append(self, latent_kv: torch.Tensor, attention_mask: torch.Tensor | None = None) -> "QuantizedMLACache":
+        b, t, l = latent_kv.shape
+        if b != self.latent_kv.shape[0] or l != self.latent_kv.shape[2]:
+            raise ValueError("new latent_kv batch and latent dim must match cache")
+        if attention_mask is not None and (tuple(attention_mask.shape) != (b, t) or attention_mask.dtype != torch.bool):
+            raise ValueError("new attention_mask must be boolean with shape [B,T]")
+        counts = None if attention_mask is None else attention_mask.sum(dim=1)
+        offsets = self.sequence_offset.clamp(max=self.latent_kv.shape[1] - 1) if t == 1 else self.sequence_offset
+        self._write(latent_kv, offsets, counts)
+        self.sequence_offset.add_(t if counts is None else counts)
+        return self
+
+    def read(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The cached latents ``[B,Tmax,L]``; slots past a row's length are zeros."""
+        if _ops.use_kernels(self.latent_kv):
+            return _ops.mla_cache_read(self.latent_kv, self.scales, self.sequence_offset, dtype=dtype)
+        values = dequantize_latents(self.latent_kv, self.scales)
+        return torch.where(self.valid_mask()[..., None], values, torch.zeros_like(values)).to(dtype)
+
+    def attend(self, query_latent: torch.Tensor, *, query_start: torch.Tensor | None = None,
+               scale: float = 1.0) -> torch.Tensor:
+        """Contexts ``[B,Tq,H,L]`` of queries absorbed into the latent space (``ops.mla_cache_attention``)."""
+        if _ops.use_kernels(query_latent):
+            return _ops.mla_cache_attention(query_latent, self.latent_kv, self.scales, self.sequence_offset,
+                                            query_start=query_start, scale=scale)
+        tq = query_latent.shape[1]
+        wd = torch.promote_types(query_latent.dtype, torch.float32)
+        start = self.sequence_offset - tq if query_start is None else query_start
+        last = start[:, None] + torch.arange(tq, device=start.device)
+        key = torch.arange(self.latent_kv.shape[1], device=start.device)
+        seen = self.valid_mask()[:, None, :] & (key <= last[..., None])  # [B,Tq,T]
+        values = self.read(wd)
+        scores = torch.einsum("bihl,btl->biht", query_latent.to(wd), values) * scale
+        scores = scores.masked_fill(~seen[:, :, None, :], -torch.inf)
+        some = seen.any(dim=-1)[:, :, None, None]
+        p = torch.softmax(torch.where(some, scores, torch.zeros_like(scores)), dim=-1)
+        p = torch.where(seen[:, :, None, :], p, torch.zeros_like(p))
+        return torch.einsum("biht,btl->bihl", p, values).to(query_latent.dtype)
+
+    def clone(self) -> "QuantizedMLACache":
+        return QuantizedMLACache(self.latent_kv.clone(), self.scales.clone(), self.sequence_offset.clone())
+
+    def reorder(self, indices: torch.Tensor) -> "QuantizedMLACache":
+        if indices.ndim != 1 or indices.dtype != torch.long:
+            raise ValueError("indices must be a rank-1 torch.long tensor")
+        return QuantizedMLACache(self.latent_kv.view(torch.uint8).index_select(0, indices).view(E4M3),
+                                 self.scales.index_select(0, indices), self.sequence_offset.index_select(0, indices))
+
+
 # --------------------------------------------------------------------------- projections
 @dataclass
 class LatentKVOutput:
@@ -389,6 +522,28 @@ def absorbed_latent_decode(query, latent_cache, cache_mask, key_up_weight, value
     return torch.einsum("bhl,hvl->bhv", ctx, wuv)[:, None]
 
 
+# Query tokens per row up to which a quantized cache is attended in the latent space.  Per cached token the
+# absorbed form costs 4 H L flops for every query token, rebuilding K and V 2 L H (Dq + Dv) once and
+# 2 H (Dq + Dv) per query token besides the traffic of K and V (and of the scores) through memory.
+ABSORBED_QUERY_LIMIT = 16
+
+
+def absorbed_quantized_attention(query, cache: QuantizedMLACache, key_up_weight, value_up_weight, num_heads, *,
+                                 query_start=None):
+    """A few query tokens ``[B,T,H,Dq]`` over the 8-bit latent cache -> ``[B,T,H,Dv]`` (fp32).
+
+    The absorbed query and the context pass between the kernels in the query's own type: the cache holds
+    four significant bits, a 16-bit rounding of either is far below that."""
+    b, t, h, dq = query.shape
+    l = cache.latent_kv.shape[-1]
+    wuk = key_up_weight.to(query.dtype).reshape(h, dq, l)
+    wuv = value_up_weight.to(query.dtype).reshape(h, -1, l)
+    q_lat = torch.bmm(query.permute(2, 0, 1, 3).reshape(h, b * t, dq), wuk).reshape(h, b, t, l).permute(1, 2, 0, 3)
+    ctx = cache.attend(q_lat, query_start=query_start, scale=1.0 / math.sqrt(dq))
+    out = torch.bmm(ctx.permute(2, 0, 1, 3).reshape(h, b * t, l), wuv.transpose(1, 2))
+    return out.reshape(h, b, t, -1).permute(1, 2, 0, 3).to(torch.promote_types(query.dtype, torch.float32))
+
+
 # --------------------------------------------------------------------------- module
 @dataclass
 class GatedMLAOutput:
@@ -487,13 +642,33 @@ class GatedMLA(nn.Module):
         prev = torch.zeros(b, dtype=torch.long, device=dev) if cache is None else cache.sequence_offset
         # The cache stores latents in the dtype the compression produces (bf16 under autocast).
         base = (MLACache.empty(b, c.kv_latent_dim, device=dev, dtype=latent.dtype) if cache is None else cache)
+        quantized = isinstance(cache, QuantizedMLACache)
         if cache is not None:
             if cache.latent_kv.shape[-1] != c.kv_latent_dim:
                 raise ValueError("cache latent dimension does not match config")
-            if cache.latent_kv.dtype != latent.dtype:
+            if cache.latent_kv.dtype != latent.dtype and not quantized:
                 latent = latent.to(cache.latent_kv.dtype)
-        updated = base.append(latent, current_mask)
-        if fast_decode:
+        if quantized:
+            # the append advances the offsets in place
+            start = prev.clone() if t > 1 else None
+            updated = cache.append(latent, attention_mask)
+            if (t <= ABSORBED_QUERY_LIMIT and not need_probs and self.absorbed_decode and not c.projection_bias
+                    and not output_diagnostics):
+                raw = absorbed_quantized_attention(query, updated, self.projections.latent_kv.key_up.weight,
+                                                   self.projections.latent_kv.value_up.weight, c.num_heads,
+                                                   query_start=start)
+                if not c.keep_attention_output_fp32:
+                    raw = raw.to(hidden_states.dtype)
+                out, gate = self._postprocess(raw, hidden_states, gate_logits)
+                if attention_mask is not None:
+                    out = out * attention_mask[..., None].to(out.dtype)
+                return GatedMLAOutput(out, updated if use_cache else None, None, None)
+            prev = updated.sequence_offset - t if start is None else start
+            latents = updated.read(latent.dtype)
+        else:
+            updated = base.append(latent, current_mask)
+            latents = updated.latent_kv
+        if fast_decode and not quantized:
             # Weight-absorbed decode: attend over the latent cache; K/V never rebuilt.
             raw = absorbed_latent_decode(query, updated.latent_kv, updated.attention_mask,
                                          self.projections.latent_kv.key_up.weight,
@@ -503,7 +678,7 @@ class GatedMLA(nn.Module):
                 raw = raw.to(hidden_states.dtype)
             out, gate = self._postprocess(raw, hidden_states, gate_logits)
             return GatedMLAOutput(out, updated if use_cache else None, None, None)
-        key, value = self.projections.reconstruct_kv(updated.latent_kv)
+        key, value = self.projections.reconstruct_kv(latents)
         self._record_qk_scale(query, key)
         qpos = prev[:, None] + torch.arange(t, device=dev)[None, :]
         cache_mask = updated.valid_mask() if isinstance(updated, StaticMLACache) else updated.attention_mask
@@ -519,13 +694,14 @@ class GatedMLA(nn.Module):
             from .diagnostics import build_mla_diagnostics
             if gate is None:
                 gate = self.output_gate.gate_values(hidden_states)
-            diagnostics = build_mla_diagnostics(query, key, value, updated.latent_kv, gate, probs,
+            diagnostics = build_mla_diagnostics(query, key, value, latents, gate, probs,
                                                 cache_mask, current_mask, updated.cache_elements,
                                                 c.full_kv_width, raw, out, self._last_qk_scale)
         return GatedMLAOutput(out, updated if use_cache else None, probs if output_attentions else None, diagnostics)
 
 
 __all__ = [
-    "GatedMLAConfig", "MLACache", "StaticMLACache", "LatentKVProjection", "LatentKVOutput", "MLAProjections", "MLAProjectionOutput",
+    "GatedMLAConfig", "MLACache", "StaticMLACache", "QuantizedMLACache", "quantize_latents", "dequantize_latents",
+    "absorbed_quantized_attention", "LatentKVProjection", "LatentKVOutput", "MLAProjections", "MLAProjectionOutput",
     "manual_causal_attention", "mla_attention", "absorbed_latent_decode", "GatedMLA", "GatedMLAOutput",
 ]

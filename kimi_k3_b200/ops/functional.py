@@ -524,6 +524,14 @@ def mla_cache_attention(query_latent, codes, scales, lengths, *, query_start=Non
     return _C().mla_cache_attention(query_latent, codes, scales, lengths, query_start, float(scale))
 
 
+def mla_cache_check() -> None:
+    """Raise if a bounded wait of an attention kernel on the current device gave up since the last check
+    (its results are void).  Waits for the device: call it where the host synchronises anyway."""
+    status = _C().mla_cache_status(True)
+    if status:
+        raise RuntimeError(f"mla_cache_attention: a bounded wait gave up (status {status}); its results are void")
+
+
 # --------------------------------------------------------------------------- sampling
 def sample_tokens(logits, seen_bits, config, seed_offset):
     """Fused next-token choice for ``[B,V]`` logits -> ``[B]`` int64 (one launch).

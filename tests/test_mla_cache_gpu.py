@@ -404,3 +404,60 @@ def test_attention_runs_of_tiles(cuda, width, rows, dtype):
     out = ops.mla_cache_attention(q, codes, scales, lens, scale=0.6)
     check_attention(out, q, codes, scales, lens, 0.6)
     assert torch.equal(out, ops.mla_cache_attention(q, codes, scales, lens, scale=0.6))
+
+
+# ------------------------------------------------------------------------------------------ through the model
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tokens", [1, 4, 16, 21])
+def test_layer_against_its_plain_form(cuda, tokens, dtype, monkeypatch):
+    """A gated-MLA layer on a quantised cache: kernels against the PyTorch form of the same layer.  Both round to
+    the layer's type at the same places but for the order of sums; a few roundings of the output's size apart."""
+    from kimi_k3_b200.models.mla import GatedMLA, GatedMLAConfig, QuantizedMLACache
+    torch.manual_seed(7)
+    layer = GatedMLA(GatedMLAConfig(d_model=640, num_heads=10, q_head_dim=64, v_head_dim=64, kv_latent_dim=640)).to(cuda).eval()
+    b, prompt, slots = 3, 70, 120
+    x0 = torch.randn(b, prompt, 640, device=cuda)
+    mask0 = torch.arange(prompt, device=cuda)[None, :] < torch.tensor([70, 33, 1], device=cuda)[:, None]
+    x = torch.randn(b, tokens, 640, device=cuda)
+    mask = torch.arange(tokens, device=cuda)[None, :] < torch.tensor([tokens, max(1, tokens // 2), 1], device=cuda)[:, None]
+    outs = []
+    for kernels in ("1", "0"):
+        monkeypatch.setenv("KIMI_K3_KERNELS", kernels)
+        with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16, enabled=dtype == torch.bfloat16):
+            pre = layer(x0, mask0, use_cache=True).cache
+            if kernels == "1":
+                first = QuantizedMLACache.from_cache(pre, slots)
+                cache = first.clone()
+            else:
+                cache = first.clone()
+            out = layer(x, None if tokens == 1 else mask, cache=cache, use_cache=True)
+        outs.append(out.hidden_states.float())
+        offsets = cache.sequence_offset.tolist()
+    assert offsets == ([71, 34, 2] if tokens == 1 else [70 + tokens, 33 + max(1, tokens // 2), 2])
+    err = (outs[0] - outs[1]).abs().max().item() / outs[1].abs().max().item()
+    assert err <= (2.0 ** -6 if dtype == torch.bfloat16 else 2.0 ** -11), err
+
+
+def test_graph_decoder_on_a_quantised_cache(cuda):
+    from kimi_k3_b200.infer import GenerationConfig, GraphDecoder
+    from kimi_k3_b200.models.mla import QuantizedMLACache
+    from test_decode_gpu import _small_model
+    model = _small_model(cuda)
+    ids = torch.randint(5, 1000, (4, 37), device=cuda)
+    mask = torch.ones_like(ids, dtype=torch.bool)
+    mask[2, 20:] = False
+    for cfg in (GenerationConfig(max_new_tokens=12),
+                GenerationConfig(max_new_tokens=12, do_sample=True, top_k=40, top_p=0.9, temperature=0.8,
+                                 repetition_penalty=1.2, seed=11)):
+        kw = dict(max_length=64, generation_config=cfg, cache_dtype=E4M3)
+        dec = GraphDecoder(model, **kw)
+        graph = dec.generate(ids, mask)
+        eager = GraphDecoder(model, use_graph=False, **kw).generate(ids, mask)
+        assert torch.equal(graph.generated_ids, eager.generated_ids)
+        assert any(isinstance(lc.state, QuantizedMLACache) for lc in graph.cache.layer_caches)
+        # a second prompt of the same shape refills the same buffers
+        ids2 = torch.randint(5, 1000, (4, 37), device=cuda)
+        captured = dec.graph
+        again = dec.generate(ids2)
+        assert dec.graph is captured
+        assert torch.equal(again.generated_ids, GraphDecoder(model, **kw).generate(ids2).generated_ids)
