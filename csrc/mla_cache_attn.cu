@@ -36,8 +36,8 @@ size_t generic_smem(int width) {
          3 * kRows * sizeof(float);
 }
 
-// fp32 arithmetic on any width and alignment: the form for fp32 queries, whose results keep fp32
-// accuracy, and for widths that the tensor-core form does not take.  A warp scores 4 tokens x 8 rows
+// fp32 arithmetic on any width and alignment: the form for what TMA cannot address (widths, strides or
+// a base that are no multiples of 16 bytes; widths under 64).  A warp scores 4 tokens x 8 rows
 // per pass over the latent axis (a lane holds four adjacent columns: 128 FMAs per 12 shared-memory
 // loads); in the context phase a thread owns four adjacent columns of up to CP groups of 1,024.
 template <typename T, int CP>

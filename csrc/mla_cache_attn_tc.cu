@@ -1,4 +1,4 @@
-// Attention over the 8-bit MLA latent cache on tcgen05 (sm_100a), bf16 and fp16 queries.
+// Attention over the 8-bit MLA latent cache on tcgen05 (sm_100a).
 //
 //   s_rt = coef_r * scale_t * sum_l q_rl code_tl        rows r = (query token, head) of one sequence
 //   o_rl = sum_t softmax_t(s)_rt * scale_t * code_tl     (a row that sees no key: zeros)
@@ -14,12 +14,13 @@
 // box row of 128 bytes serves as a K-major row of the first product and as an MN-major row of the
 // second.  O^T stays in TMEM for a whole sequence segment (L / 128 accumulators of `rows` columns).
 //
-// Splitting into 8-bit parts keeps 16-bit accuracy.  A query row is scaled by a power of two to
-// [128, 256) and written as q = q0 + q1 / 32 + q2 / 1024 in e4m3, each part the rounding of what the
-// one before left (5 bits a part): two parts hold every bf16, three every fp16 within 2^-17 of the
-// row's maximum.  The parts sit side by side on N (A is read once) and are added in fp32.  The weights
+// Splitting into 8-bit parts keeps the query type's accuracy.  A query row is scaled by a power of two to
+// [128, 256) and written as q = q0 + q1 / 32 + q2 / 1024 + .. in e4m3, each part the rounding of what the
+// one before left (5 bits a part): two parts hold every bf16, three every fp16, five every fp32 but for
+// what lies more than 2^-18, 2^-27, 2^-38 below the row's maximum.  The parts sit side by side on N (A is read once) and are added in fp32.  The weights
 // v = 2^(s + log2(scale_t) - ref) <= 2^15 are split into e5m2 parts (3 + 4 + 4 + .. bits) along K, all
-// accumulating into the same columns: three for bf16 outputs (11 bits), four for fp16 (14 bits).  e5m2
+// accumulating into the same columns: three for bf16 outputs (11 bits), four for fp16 (14), six for fp32
+// (22).  e5m2
 // because of its range: the parts of a weight 2^-18 below the row's reference are still whole, where
 // e4m3's step of 2^-9 would cut what many small weights add up to.
 //
@@ -63,8 +64,12 @@ constexpr int kMaxGroup = 6;               // boxes of a stage
 constexpr int kSmemMax = 227 * 1024;
 constexpr int kMaxGrid = 256;              // CTAs of the attention kernel
 constexpr int kOcts = 8;                   // 8-element pieces of a query row per lane: widths up to 2,048
+constexpr int kMisaligned = 9;             // status: shared memory off a 1,024-byte boundary
 constexpr float kTop = 15.f;               // a weight may reach 2^kTop
-constexpr float kRoom = 6.f;               // a new reference leaves this many bits
+// a new reference leaves this many bits: fewer moves of the accumulators against a lower floor of the weights
+// (2^-26 of the largest; 2^-31 for fp32 results)
+template <int QP>
+constexpr float kRoom = QP == 5 ? 1.f : 6.f;
 constexpr float kNoRef = -3e38f;            // finite: a score of -inf weighs nothing against it
 constexpr float kSumRoom = 40.f;           // the sums' reference may lag by this many bits
 
@@ -81,6 +86,7 @@ struct Plan {
   int runs = 0;        // context products of a box: ceil(parts / stack)
   int ns = 0, np = 0;  // N of the score and of the context product
   int p_bytes = 0;     // one weight buffer
+  int p_bufs = 2;
   int ahead = 0;       // stages of the next tile's scores issued before this tile's context product
   uint32_t tmem = 0;
   size_t smem = 0;
@@ -94,7 +100,7 @@ struct TcParams {
   int rows, rows_tile, row_tiles, boxes, group, tile_stages, stages, s_bufs, ahead, direct, t_first, q_vec;
   int wide;            // one copy per stage (L a multiple of 128), else one per box
   int fetch;           // tiles ahead that are brought into L2
-  int r_pad, stack, runs, ns, np, p_bytes, q_bytes, grid;
+  int r_pad, stack, runs, ns, np, p_bytes, p_bufs, q_bytes, grid;
   uint32_t tmem;
   int64_t z_mul;       // 0 when every sequence reads the same cache rows
   uint8_t* q_parts;    // [pairs][q_bytes]: the shared-memory image of a pair's query parts
@@ -310,6 +316,11 @@ struct Walk {
   }
 };
 
+template <typename T>
+struct alignas(16) Oct8 {
+  T v[8];
+};
+
 // Query parts, one warp per row.
 template <typename T, int QP>
 __global__ void __launch_bounds__(256) attn_tc_prep_kernel(const __grid_constant__ TcParams p) {
@@ -327,28 +338,27 @@ __global__ void __launch_bounds__(256) attn_tc_prep_kernel(const __grid_constant
   const int qi = qr / p.a.heads, h = qr - qi * p.a.heads;
   const T* q = static_cast<const T*>(p.a.q) + b * p.a.q_b + qi * p.a.q_i + h * p.a.q_h;
   const int octs = p.a.cache.width >> 3;
-  int4 x[kOcts];
-  uint32_t top = 0;
+  Oct8<T> x[kOcts];
+  uint32_t top = 0;  // of the magnitudes' bits, which order like the values; infinities and NaN on top
 #pragma unroll
   for (int i = 0; i < kOcts; ++i) {
     const int o = lane + 32 * i;
-    x[i] = make_int4(0, 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[i].v[j] = from_f<T>(0.f);
     if (o < octs) {
       if (p.q_vec) {
-        x[i] = __ldg(reinterpret_cast<const int4*>(q) + o);
-      } else {
-        Vec<T> e;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) e.v[j] = q[o * 8 + j];
-        x[i] = *reinterpret_cast<const int4*>(e.v);
+        for (int j = 0; j < (int)sizeof(T) / 2; ++j)
+          reinterpret_cast<int4*>(x[i].v)[j] = __ldg(reinterpret_cast<const int4*>(q + o * 8) + j);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[i].v[j] = q[o * 8 + j];
       }
     }
-    const uint32_t m = 0x7FFF7FFFu;
-    top = __vmaxu2(__vmaxu2(top, __vmaxu2(x[i].x & m, x[i].y & m)), __vmaxu2(x[i].z & m, x[i].w & m));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(to_f<T>(x[i].v[j])) & 0x7FFFFFFFu);
   }
-  top = __reduce_max_sync(0xffffffffu, max(top & 0xFFFFu, top >> 16));
-  const unsigned short top16 = (unsigned short)top;
-  top = __float_as_uint(to_f<T>(*reinterpret_cast<const T*>(&top16)));
+  top = __reduce_max_sync(0xffffffffu, top);
   const bool bad = top >= 0x7F800000u;
   const int k = bad ? 0 : min(126, 134 - (int)(top >> 23));  // the maximum to [128, 256)
   const float f = pow2i(k);
@@ -357,11 +367,9 @@ __global__ void __launch_bounds__(256) attn_tc_prep_kernel(const __grid_constant
   for (int i = 0; i < kOcts; ++i) {
     const int o = lane + 32 * i;
     if (o >= p.boxes * 16) break;
-    Vec<T> e;
-    *reinterpret_cast<int4*>(e.v) = x[i];
     float y[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = bad ? 0.f : e.f(j) * f;
+    for (int j = 0; j < 8; ++j) y[j] = bad ? 0.f : to_f<T>(x[i].v[j]) * f;
     uint8_t* at = image + (size_t)(o >> 4) * NS * 128 + (o & 1) * 8;
 #pragma unroll
     for (int part = 0; part < QP; ++part) {
@@ -385,11 +393,15 @@ template <typename T, int RH, int QP>
 __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_constant__ TcParams p) {
   using S = Shape<RH, QP>;
   constexpr int R = S::R, HR = RH / 2;  // a thread of a compute group handles HR rows of one token
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* ring = smem_raw + ((1024u - (tc::smem_u32(smem_raw) & 1023u)) & 1023u);  // [stages][group][kBox]
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* ring = smem_raw;                                   // [stages][group][kBox]
+  if (tc::smem_u32(smem_raw) & 1023u) {  // the swizzle needs it; no static shared memory is in front
+    if (threadIdx.x == 0) atomicCAS(p.status, 0, kMisaligned);
+    return;
+  }
   uint8_t* sq = ring + (size_t)p.stages * p.group * kBox;     // [boxes][NS][128] query parts
-  uint8_t* sp = sq + p.q_bytes;                               // [2][p_bytes] weight parts
-  float2* sfac = reinterpret_cast<float2*>(sp + 2 * p.p_bytes);  // [R] normalisation of a row
+  uint8_t* sp = sq + p.q_bytes;                               // [p_bufs][p_bytes] weight parts
+  float2* sfac = reinterpret_cast<float2*>(sp + p.p_bufs * p.p_bytes);  // [R] normalisation of a row
   float* sref = reinterpret_cast<float*>(sfac + R);           // [R] weight references
   float* sreft = sref + R;                                    // [R] sum references
   float* sdel = sreft + R;                                    // [R] change of a weight reference
@@ -429,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     tc::tma_prefetch(&p.map);
   }
   // a context product may read weight parts that no row has: zeros
-  for (int i = tid; i < 2 * p.p_bytes / 16; i += kThreads) reinterpret_cast<int4*>(sp)[i] = make_int4(0, 0, 0, 0);
+  for (int i = tid; i < p.p_bufs * p.p_bytes / 16; i += kThreads) reinterpret_cast<int4*>(sp)[i] = make_int4(0, 0, 0, 0);
   tc::fence_barrier_init();
   tc::fence_proxy_async();
   pdl_launch();
@@ -562,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         const uint32_t pb = o_n & 1;
         if (mbar_over(&p_full[pb], o_n >> 1)) {
           tc::tc_fence_after();
-          const uint32_t pd = (uint32_t)bd_p + pb * (uint32_t)(p.p_bytes >> 4);
+          const uint32_t pd = (uint32_t)bd_p + (p.p_bufs == 2 ? pb : 0) * (uint32_t)(p.p_bytes >> 4);
           uint32_t d = tmem;
           for (int i = 0; i < p.tile_stages; ++i) {
             const int nb = min(p.group, p.boxes - i * p.group);
@@ -765,7 +777,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             const float ms = fmaxf(fmaxf(sred[4 * R + r], sred[5 * R + r]), fmaxf(sred[6 * R + r], sred[7 * R + r]));
             float del = 0.f, mul = 1.f;
             if (ma > sref[r] + kTop) {
-              const float to = ceilf(ma) - (kTop - kRoom);
+              const float to = ceilf(ma) - (kTop - kRoom<QP>);
               del = sref[r] - to;
               sref[r] = to;
             }
@@ -814,9 +826,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             if (waited) tmem_wait_st();
           }
         }
-        // weights into parts; the buffer was last read by the context product of two tiles ago
-        if (n_tile >= 2) wait(&pv_done[pb], (n_tile >> 1) - 1, tc::kTimeoutTmemEmpty);
-        uint8_t* wp = sp + pb * p.p_bytes;
+        // weights into parts; the buffer was last read by the context product of p_bufs tiles ago
+        const uint32_t before = n_tile - p.p_bufs;
+        if (n_tile >= (uint32_t)p.p_bufs) wait(&pv_done[before & 1], before >> 1, tc::kTimeoutTmemEmpty);
+        uint8_t* wp = sp + (p.p_bufs == 2 ? pb : 0) * p.p_bytes;
 #pragma unroll
         for (int r = 0; r < HR; r += 2) {
           float v[2];
@@ -825,16 +838,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             sum[r + e] += ex2(es[r + e]);
             v[e] = ex2(ev[r + e]);
           }
-          // fp16 holds three parts; with four, the first comes off in fp32
+          // fp16 holds three parts; those before come off in fp32
           __half2 h;
           if constexpr (S::WP == 3) h = __floats2half2_rn(v[0], v[1]);
 #pragma unroll
           for (int part = 0; part < S::WP; ++part) {
             uint32_t c;
-            if (S::WP > 3 && part == 0) {
+            if (part < S::WP - 3) {
               c = __nv_cvt_float2_to_fp8x2(make_float2(v[0], v[1]), __NV_SATFINITE, __NV_E5M2);
               const float2 d = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)c, __NV_E5M2)));
-              h = __floats2half2_rn(v[0] - d.x, v[1] - d.y);
+              v[0] -= d.x;
+              v[1] -= d.y;
+              if (part == S::WP - 4) h = __floats2half2_rn(v[0], v[1]);
             } else {
               c = take_e5m2x2(h);
             }
@@ -1018,10 +1033,12 @@ __global__ void __launch_bounds__(256) attn_tc_join_kernel(const __grid_constant
   const float inv = sum != 0.f ? 1.f / sum : 0.f;
   T* out = static_cast<T*>(p.a.out) + ((int64_t)b * p.rows + row0 + r) * width + l;
   const float o[4] = {acc.x, acc.y, acc.z, acc.w};
-  T t[4];
+  struct alignas(4 * sizeof(T)) Four {
+    T t[4];
+  } four;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) t[i] = from_f<T>(inv == 0.f ? 0.f : o[i] * inv);
-  *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(t);
+  for (int i = 0; i < 4; ++i) four.t[i] = from_f<T>(inv == 0.f ? 0.f : o[i] * inv);
+  *reinterpret_cast<Four*>(out) = four;
 }
 
 // Weight parts on N cost accumulator columns, parts along K cost a pass over the tile (36 + N / 5 clocks
@@ -1038,18 +1055,22 @@ bool fit(int boxes, Plan* pl) {
     const int cost = runs * (36 * 5 + np);
     if (found && cost >= best && bufs <= pl->s_bufs) continue;
     const int p_bytes = np * 128 * ((runs + 1) / 2);
-    const size_t fixed = (size_t)boxes * S::NS * 128 + 2 * p_bytes + (2 + 4 + 8) * S::R * 4 +
-                         (2 * kMaxStages + 10) * 8 + 64 + 1024;  // + alignment
-    if (fixed >= kSmemMax) continue;
     // Stages as wide as the ring allows with a tile in it and more to load: a wide stage reads long pieces of
-    // each cached row together.
-    int tile_stages = 0, group = 0, stages = 0;
-    for (int g = kMaxGroup; g >= 1; --g) {
-      tile_stages = (boxes + g - 1) / g;
-      group = (boxes + tile_stages - 1) / tile_stages;
-      stages = (int)((kSmemMax - fixed) / (group * kBox));
-      stages = stages < kMaxStages ? stages : kMaxStages;
-      if (stages > tile_stages) break;
+    // each cached row together.  Where the ring holds less than two tiles, a tile's weights are written only
+    // once the tile before has left the ring: one weight buffer then costs no time and widens the ring.
+    int tile_stages = 0, group = 0, stages = 0, p_bufs = 2;
+    size_t fixed = 0;
+    for (; p_bufs >= 1; --p_bufs) {
+      fixed = (size_t)boxes * S::NS * 128 + p_bufs * p_bytes + (2 + 4 + 8) * S::R * 4 + (2 * kMaxStages + 10) * 8 + 64;
+      stages = 0;
+      for (int g = kMaxGroup; g >= 1 && fixed < kSmemMax; --g) {
+        tile_stages = (boxes + g - 1) / g;
+        group = (boxes + tile_stages - 1) / tile_stages;
+        stages = (int)((kSmemMax - fixed) / (group * kBox));
+        stages = stages < kMaxStages ? stages : kMaxStages;
+        if (stages > tile_stages) break;
+      }
+      if (stages >= 2 * tile_stages || p_bufs == 1) break;
     }
     if (stages <= tile_stages) continue;
     found = true;
@@ -1065,6 +1086,7 @@ bool fit(int boxes, Plan* pl) {
     pl->runs = runs;
     pl->np = np;
     pl->p_bytes = p_bytes;
+    pl->p_bufs = p_bufs;
     pl->ahead = stages - tile_stages < tile_stages ? stages - tile_stages : tile_stages;
     uint32_t n = 32;
     while (n < (uint32_t)(cols + bufs * S::NS)) n *= 2;
@@ -1111,7 +1133,7 @@ bool make_plan(const MlaCacheAttnArgs& a, Plan* pl) {
 }
 
 bool plan_for(int dtype, const MlaCacheAttnArgs& a, Plan* pl) {
-  return dtype == 1 ? make_plan<2>(a, pl) : make_plan<3>(a, pl);
+  return dtype == 0 ? make_plan<5>(a, pl) : dtype == 1 ? make_plan<2>(a, pl) : make_plan<3>(a, pl);
 }
 
 // wide: [B][L / 128][Tmax][128] as a view of the cache, boxes of `group` chunks x 64 tokens.  Else [B][Tmax][L]
@@ -1206,9 +1228,9 @@ cudaError_t launch_rh(const TcParams& p, const Plan& pl, cudaStream_t s) {
 
 }  // namespace
 
-// 16-bit queries, and code rows that TMA can address: 16-byte base and strides.
+// Code rows that TMA can address: 16-byte base and strides.
 bool mla_attn_tc_supported(int dtype, const MlaCacheAttnArgs& a) {
-  if (dtype != 1 && dtype != 2) return false;
+  if (dtype < 0 || dtype > 2) return false;
   if (a.cache.width % 16 || a.cache.width < 64 || a.cache.width > 256 * kOcts || a.cache.slots > (1 << 30)) return false;
   if ((reinterpret_cast<uintptr_t>(a.cache.codes) & 15) || (a.batch > 1 && a.cache.code_b % 16)) return false;
   if (a.cache.slots > 1 && (a.cache.code_t % 16 || a.cache.code_t < a.cache.width)) return false;
@@ -1258,12 +1280,14 @@ cudaError_t mla_attn_tc(int dtype, const MlaCacheAttnArgs& a, cudaStream_t s) {
   p.ns = pl.ns;
   p.np = pl.np;
   p.p_bytes = pl.p_bytes;
+  p.p_bufs = pl.p_bufs;
   p.q_bytes = pl.boxes * pl.ns * 128;
   p.grid = pl.grid;
   p.fetch = kFetch;
   p.direct = pl.direct ? 1 : 0;
   p.tmem = pl.tmem;
-  p.q_vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.q_b % 8 == 0 && a.q_i % 8 == 0 && a.q_h % 8 == 0;
+  const int vec = dtype == 0 ? 4 : 8;
+  p.q_vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.q_b % vec == 0 && a.q_i % vec == 0 && a.q_h % vec == 0;
   const bool one = a.batch == 1 || a.cache.code_b == 0;  // every sequence reads the same rows
   p.z_mul = one ? 0 : 1;
   p.t_first = one || p.a.cache.code_t <= a.cache.code_b ? 1 : 0;
@@ -1283,7 +1307,11 @@ cudaError_t mla_attn_tc(int dtype, const MlaCacheAttnArgs& a, cudaStream_t s) {
   p.prefix = reinterpret_cast<int*>(a.part_acc + wk.prefix);
   p.status = status_ptr();
   if (!p.status) return cudaErrorInvalidValue;
-  return dtype == 1 ? launch_rh<__nv_bfloat16, 2>(p, pl, s) : launch_rh<__half, 3>(p, pl, s);
+  switch (dtype) {
+    case 0: return launch_rh<float, 5>(p, pl, s);
+    case 1: return launch_rh<__nv_bfloat16, 2>(p, pl, s);
+    default: return launch_rh<__half, 3>(p, pl, s);
+  }
 }
 
 int* mla_cache_default_status() { return status_ptr(); }

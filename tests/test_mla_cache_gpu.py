@@ -388,7 +388,7 @@ def test_refusals(cuda):
     assert not ops.mla_cache_attention(q.detach(), codes[:, :0], scales[:, :0], n).any()
 
 
-@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("rows", [(1, 3), (2, 8), (3, 8), (4, 8), (1, 24), (4, 12), (5, 10), (6, 12)],
                          ids=lambda r: "x".join(map(str, r)))
 @pytest.mark.parametrize("width", [128, 640, 768, 1536])
