@@ -72,6 +72,15 @@ struct Oct<float> {
   static KIMI_D uint32_t bits(uint32_t t) { return t; }
 };
 
+// Sequence and token of a row; the launchers bound the rows by 2^31 (a 64-bit division is ten times a 32-bit one).
+KIMI_D bool row_of(int64_t tokens, int batch, int* b, int64_t* j) {
+  const uint32_t row = blockIdx.x * kRowWarps + (threadIdx.x >> 5), t = (uint32_t)tokens;
+  const uint32_t q = row / t;
+  *b = (int)q;
+  *j = row - q * t;
+  return q < (uint32_t)batch;
+}
+
 // Slot of token j of sequence b, or -1.
 KIMI_D int64_t write_slot(const MlaCacheWriteArgs& a, int b, int64_t j) {
   if (a.counts.p && j >= get(a.counts, b)) return -1;
@@ -83,10 +92,9 @@ KIMI_D int64_t write_slot(const MlaCacheWriteArgs& a, int b, int64_t j) {
 template <typename T, int OCTS>
 __global__ void __launch_bounds__(kRowWarps * 32) write_kernel(const __grid_constant__ MlaCacheWriteArgs a) {
   const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
-  if (row >= (int64_t)a.batch * a.tokens) return;
-  const int b = (int)(row / a.tokens);
-  const int64_t j = row - (int64_t)b * a.tokens;
+  int b;
+  int64_t j;
+  if (!row_of(a.tokens, a.batch, &b, &j)) return;
   const int64_t slot = write_slot(a, b, j);
   if (slot < 0) return;
   const T* x = static_cast<const T*>(a.x) + b * a.x_b + j * a.x_t;
@@ -125,10 +133,9 @@ __global__ void __launch_bounds__(kRowWarps * 32) write_kernel(const __grid_cons
 template <typename T>
 __global__ void __launch_bounds__(kRowWarps * 32) write_any_kernel(const __grid_constant__ MlaCacheWriteArgs a) {
   const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
-  if (row >= (int64_t)a.batch * a.tokens) return;
-  const int b = (int)(row / a.tokens);
-  const int64_t j = row - (int64_t)b * a.tokens;
+  int b;
+  int64_t j;
+  if (!row_of(a.tokens, a.batch, &b, &j)) return;
   const int64_t slot = write_slot(a, b, j);
   if (slot < 0) return;
   const T* x = static_cast<const T*>(a.x) + b * a.x_b + j * a.x_t;
@@ -147,14 +154,13 @@ __global__ void __launch_bounds__(kRowWarps * 32) write_any_kernel(const __grid_
 template <typename T, bool OCT>
 __global__ void __launch_bounds__(kRowWarps * 32) read_kernel(const __grid_constant__ MlaCacheReadArgs a) {
   const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
-  if (row >= (int64_t)a.batch * a.tokens) return;
-  const int b = (int)(row / a.tokens);
-  const int64_t j = row - (int64_t)b * a.tokens;
+  int b;
+  int64_t j;
+  if (!row_of(a.tokens, a.batch, &b, &j)) return;
   const bool live = !a.lengths.p || j < get(a.lengths, b);
   const uint8_t* c = a.cache.codes + b * a.cache.code_b + j * a.cache.code_t;
   const float s = live ? a.cache.scales[b * a.cache.scale_b + j * a.cache.scale_t] : 0.f;
-  T* y = static_cast<T*>(a.out) + row * a.cache.width;
+  T* y = static_cast<T*>(a.out) + ((int64_t)b * a.tokens + j) * a.cache.width;
   if constexpr (OCT) {
     const int octs = a.cache.width >> 3;
 #pragma unroll 4
@@ -188,7 +194,7 @@ bool aligned(const void* p, int64_t to) { return (reinterpret_cast<uintptr_t>(p)
 template <typename T>
 cudaError_t launch_write(const MlaCacheWriteArgs& a, cudaStream_t s) {
   const int64_t rows = (int64_t)a.batch * a.tokens, grid = (rows + kRowWarps - 1) / kRowWarps;
-  if (grid > 0x7FFFFFFF) return cudaErrorInvalidValue;
+  if (rows > 0x7FFFFFF0) return cudaErrorInvalidValue;
   const int64_t eb = a.x_b * (int64_t)sizeof(T), et = a.x_t * (int64_t)sizeof(T);
   const bool oct = a.cache.width % 8 == 0 && aligned(a.x, 16) && eb % 16 == 0 && et % 16 == 0 &&
                    aligned(a.cache.codes, 8) && a.cache.code_b % 8 == 0 && a.cache.code_t % 8 == 0;
@@ -211,7 +217,7 @@ cudaError_t launch_write(const MlaCacheWriteArgs& a, cudaStream_t s) {
 template <typename T>
 cudaError_t launch_read(const MlaCacheReadArgs& a, cudaStream_t s) {
   const int64_t rows = (int64_t)a.batch * a.tokens, grid = (rows + kRowWarps - 1) / kRowWarps;
-  if (grid > 0x7FFFFFFF) return cudaErrorInvalidValue;
+  if (rows > 0x7FFFFFF0) return cudaErrorInvalidValue;
   const bool oct = a.cache.width % 8 == 0 && aligned(a.cache.codes, 8) && a.cache.code_b % 8 == 0 &&
                    a.cache.code_t % 8 == 0 && aligned(a.out, 16);
   if (oct) read_kernel<T, true><<<(unsigned)grid, kRowWarps * 32, 0, s>>>(a);

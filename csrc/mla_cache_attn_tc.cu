@@ -34,7 +34,7 @@
 // others leave a normalised context and its log-sum, joined by a second kernel in a fixed order.
 //
 // Three launches, each started while the one before still runs (programmatic dependent launch): the
-// query parts and the split of the tile list; the attention; the join.  The query parts are written as
+// query parts; the attention, each CTA of which finds its own range of the list; the join.  The query parts are written as
 // the image of their shared-memory tile, so that a CTA brings in the next sequence's queries with one
 // bulk copy while it still works on the last tile of this one.
 //
@@ -43,6 +43,7 @@
 // Every mbarrier wait is bounded and reports through the status word.
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <mutex>
 
 #include "device_info.h"
@@ -60,7 +61,7 @@ constexpr int kBox = kTile * 128;          // bytes of a box
 constexpr int kThreads = 320;
 constexpr int kMaxStages = 32;             // of the ring
 constexpr int kFetch = 1;                  // tiles ahead that are brought into L2
-constexpr int kMaxGroup = 6;               // boxes of a stage
+constexpr int kMaxGroup = 8;               // boxes of a stage
 constexpr int kSmemMax = 227 * 1024;
 constexpr int kMaxGrid = 256;              // CTAs of the attention kernel
 constexpr int kOcts = 8;                   // 8-element pieces of a query row per lane: widths up to 2,048
@@ -87,7 +88,6 @@ struct Plan {
   int ns = 0, np = 0;  // N of the score and of the context product
   int p_bytes = 0;     // one weight buffer
   int p_bufs = 2;
-  int ahead = 0;       // stages of the next tile's scores issued before this tile's context product
   uint32_t tmem = 0;
   size_t smem = 0;
   bool direct = false;  // one CTA per pair, nothing to join
@@ -97,7 +97,7 @@ struct Plan {
 struct TcParams {
   CUtensorMap map;
   MlaCacheAttnArgs a;
-  int rows, rows_tile, row_tiles, boxes, group, tile_stages, stages, s_bufs, ahead, direct, t_first, q_vec;
+  int rows, rows_tile, row_tiles, boxes, group, tile_stages, stages, s_bufs, direct, t_first, q_vec;
   int wide;            // one copy per stage (L a multiple of 128), else one per box
   int fetch;           // tiles ahead that are brought into L2
   int r_pad, stack, runs, ns, np, p_bytes, p_bufs, q_bytes, grid;
@@ -1087,13 +1087,25 @@ bool fit(int boxes, Plan* pl) {
     pl->np = np;
     pl->p_bytes = p_bytes;
     pl->p_bufs = p_bufs;
-    pl->ahead = stages - tile_stages < tile_stages ? stages - tile_stages : tile_stages;
     uint32_t n = 32;
     while (n < (uint32_t)(cols + bufs * S::NS)) n *= 2;
     pl->tmem = n;
     pl->smem = fixed + (size_t)stages * group * kBox;
   }
   return found;
+}
+
+// Whether each pair is one CTA's, written without a join.  Against the split list that gives up balance (all of
+// `tiles` in a row, a whole wave of CTAs more for a pair too many) and saves the parts' way through memory and
+// a launch.  In ns, as measured: 1.2 a tile and latent, 2,000 the join, 1 / 3,000 a byte of the parts, there and back.
+// One CTA a pair / split, bf16: 64 x 256 tokens, 16 heads, L 1024 15.0 / 20.4 us; 100 x 400, 10, 640 18.1 / 24.9;
+// 32 x 128, 12, 768 10.1 / 11.9; 200 x 500, 10, 640 35.2 / 35.9; 16 x 528, 10, 640 18.7 / 16.2; 4 x 300, 24, 1536
+// 31.7 / 24.6; 1 x 512, 10, 640 16.5 / 12.7.  From the slots: the lengths are on the device.
+bool one_cta_per_pair(int64_t pairs, int64_t tiles, int sms, int rows, int width) {
+  const int64_t whole = (pairs + sms - 1) / sms * (tiles + kStart);
+  const int64_t split = std::max<int64_t>((pairs * (tiles + kStart) + sms - 1) / sms, 1 + kStart);
+  const int64_t part_bytes = std::min<int64_t>(pairs * tiles, sms) * rows * width * 8;
+  return (whole - split) * width * 6 / 5 <= 2000 + part_bytes / 3000;
 }
 
 // Rows of a CTA: the fewest padded rows that hold them all, else as many as fit TMEM and shared memory
@@ -1127,7 +1139,7 @@ bool make_plan(const MlaCacheAttnArgs& a, Plan* pl) {
   const int64_t pairs = (int64_t)a.batch * pl->row_tiles, tiles = (a.cache.slots + kTile - 1) / kTile;
   if (pairs > (1 << 20) || pairs * tiles > (1 << 29)) return false;
   const int sms = device_sms() < kMaxGrid ? device_sms() : kMaxGrid;
-  pl->direct = tiles == 1;
+  pl->direct = one_cta_per_pair(pairs, tiles, sms, pl->rows_tile, a.cache.width);
   pl->grid = pl->direct ? (int)pairs : (int)(pairs * tiles < sms ? pairs * tiles : sms);
   return true;
 }
@@ -1273,7 +1285,6 @@ cudaError_t mla_attn_tc(int dtype, const MlaCacheAttnArgs& a, cudaStream_t s) {
   p.tile_stages = pl.tile_stages;
   p.stages = pl.stages;
   p.s_bufs = pl.s_bufs;
-  p.ahead = pl.ahead;
   p.stack = pl.stack;
   p.runs = pl.runs;
   p.r_pad = 2 * pl.rh;

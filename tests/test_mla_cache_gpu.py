@@ -406,6 +406,19 @@ def test_attention_runs_of_tiles(cuda, width, rows, dtype):
     assert torch.equal(out, ops.mla_cache_attention(q, codes, scales, lens, scale=0.6))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("case", [(32, 1, 12, 768, 128), (64, 1, 16, 1024, 256), (100, 1, 10, 640, 400),
+                                  (320, 1, 3, 512, 250), (40, 5, 10, 640, 190)], ids=lambda c: "x".join(map(str, c)))
+def test_attention_many_short_sequences(cuda, case, dtype):
+    """Batches that fill the GPU with one sequence each, in one wave or several; empty sequences among them."""
+    from kimi_k3_b200 import ops
+    b, tq, h, width, slots = case
+    codes, scales = make_cache(b, slots, width, cuda)
+    q = queries(b, tq, h, width, dtype, cuda)
+    lens = torch.tensor([(i * 89) % (slots + 1) if i % 4 else (0, 1, 64, 65, slots)[i // 4 % 5] for i in range(b)], device=cuda)
+    check_attention(ops.mla_cache_attention(q, codes, scales, lens, scale=0.6), q, codes, scales, lens, 0.6)
+
+
 # ------------------------------------------------------------------------------------------ through the model
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("tokens", [1, 4, 16, 21])
