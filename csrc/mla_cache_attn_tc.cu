@@ -64,7 +64,9 @@ constexpr int kFetch = 1;                  // tiles ahead that are brought into 
 constexpr int kMaxGroup = 8;               // boxes of a stage
 constexpr int kSmemMax = 227 * 1024;
 constexpr int kMaxGrid = 256;              // CTAs of the attention kernel
-constexpr int kOcts = 8;                   // 8-element pieces of a query row per lane: widths up to 2,048
+template <int SL>
+constexpr int kJoinThreads = SL == 1 ? 128 : 256;
+constexpr int kPrepThreads = 256;          // 8 elements of a query row each: widths up to 2,048
 constexpr int kMisaligned = 9;             // status: shared memory off a 1,024-byte boundary
 constexpr float kTop = 15.f;               // a weight may reach 2^kTop
 // a new reference leaves this many bits: fewer moves of the accumulators against a lower floor of the weights
@@ -101,6 +103,7 @@ struct TcParams {
   int wide;            // one copy per stage (L a multiple of 128), else one per box
   int fetch;           // tiles ahead that are brought into L2
   int r_pad, stack, runs, ns, np, p_bytes, p_bufs, q_bytes, grid;
+  int start;           // places of a pair in front of its tiles (see kStart)
   uint32_t tmem;
   int64_t z_mul;       // 0 when every sequence reads the same cache rows
   uint8_t* q_parts;    // [pairs][q_bytes]: the shared-memory image of a pair's query parts
@@ -119,7 +122,6 @@ struct Shape {
   static constexpr int NS = pad16(QP * R);  // N of the score product
   static constexpr int WP = QP + 1;
   static constexpr int MAX_STACK = RH <= 8 ? WP : RH <= 12 ? 3 : 2;  // registers of the epilogue
-  static constexpr int EPI_BOXES = MAX_STACK * RH <= 16 ? 3 : MAX_STACK * RH <= 24 ? 2 : 1;
 };
 
 KIMI_D bool elect_one() {
@@ -292,7 +294,8 @@ KIMI_D int pair_tiles(const TcParams& p, int v, int64_t* len_out, int64_t* start
 }
 
 // The list of all pairs' tiles is cut into equal ranges, one per CTA.  Starting a pair costs a CTA about as
-// much as kStart tiles (an epilogue, an empty pipeline), so each pair with tiles has kStart places in front.
+// much as kStart tiles (an epilogue, an empty pipeline), so each pair with tiles has kStart places in front;
+// none where every tile can have its own CTA.
 constexpr int kStart = 2;
 
 // This CTA's share of the list, walked pair by pair (every role walks it on its own).
@@ -306,7 +309,7 @@ struct Walk {
       if (skip < tiles) {
         t0 = skip;
         t1 = min(tiles, skip + left);
-        left -= t1 - t0 + kStart;  // the next pair's places in front
+        left -= t1 - t0 + p.start;  // the next pair's places in front
         skip = 0;
         return true;
       }
@@ -321,56 +324,50 @@ struct alignas(16) Oct8 {
   T v[8];
 };
 
-// Query parts, one warp per row.
+// Query parts, one block per row and one thread per 8 elements.  64 x 24 rows of 1,536 in bf16 (4.7 MB in, 4.7 MB
+// out) take 4.4 us, most of it a launch, one trip to memory and one back; a warp per row took 5.6, its long code
+// fetched cold, and the attention kernel gets its SMs only behind it.
 template <typename T, int QP>
-__global__ void __launch_bounds__(256) attn_tc_prep_kernel(const __grid_constant__ TcParams p) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int pairs = p.a.batch * p.row_tiles, R = p.r_pad, NS = p.ns;
+__global__ void __launch_bounds__(kPrepThreads) attn_tc_prep_kernel(const __grid_constant__ TcParams p) {
+  __shared__ uint32_t stop[kPrepThreads / 32];
+  const int o = threadIdx.x, warp = o >> 5, R = p.r_pad, NS = p.ns;
+  const int v = blockIdx.x / p.rows_tile, r = blockIdx.x - v * p.rows_tile;
+  const int b = v / p.row_tiles, qr = (v - b * p.row_tiles) * p.rows_tile + r;
+  const int qi = qr / p.a.heads, h = qr - qi * p.a.heads;
   pdl_wait();
   // only now: the attention kernel reads cache and lengths without waiting for this one to end, so it may
   // not start before everything ahead of this kernel is done
   pdl_launch();
-  const int row = blockIdx.x * 8 + warp;
-  if (row >= pairs * p.rows_tile) return;
-  const int v = row / p.rows_tile, r = row - v * p.rows_tile;
-  const int b = v / p.row_tiles, qr = (v - b * p.row_tiles) * p.rows_tile + r;
   if (qr >= p.rows) return;
-  const int qi = qr / p.a.heads, h = qr - qi * p.a.heads;
-  const T* q = static_cast<const T*>(p.a.q) + b * p.a.q_b + qi * p.a.q_i + h * p.a.q_h;
-  const int octs = p.a.cache.width >> 3;
-  Oct8<T> x[kOcts];
+  const T* q = static_cast<const T*>(p.a.q) + b * p.a.q_b + qi * p.a.q_i + h * p.a.q_h + o * 8;
+  Oct8<T> x;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x.v[j] = from_f<T>(0.f);
+  if (o < p.a.cache.width >> 3) {
+    if (p.q_vec) {
+#pragma unroll
+      for (int j = 0; j < (int)sizeof(T) / 2; ++j)
+        reinterpret_cast<int4*>(x.v)[j] = __ldg(reinterpret_cast<const int4*>(q) + j);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x.v[j] = q[j];
+    }
+  }
   uint32_t top = 0;  // of the magnitudes' bits, which order like the values; infinities and NaN on top
 #pragma unroll
-  for (int i = 0; i < kOcts; ++i) {
-    const int o = lane + 32 * i;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[i].v[j] = from_f<T>(0.f);
-    if (o < octs) {
-      if (p.q_vec) {
-#pragma unroll
-        for (int j = 0; j < (int)sizeof(T) / 2; ++j)
-          reinterpret_cast<int4*>(x[i].v)[j] = __ldg(reinterpret_cast<const int4*>(q + o * 8) + j);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[i].v[j] = q[o * 8 + j];
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(to_f<T>(x[i].v[j])) & 0x7FFFFFFFu);
-  }
+  for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(to_f<T>(x.v[j])) & 0x7FFFFFFFu);
   top = __reduce_max_sync(0xffffffffu, top);
+  if ((o & 31) == 0) stop[warp] = top;
+  __syncthreads();
+  for (int i = 0; i < (int)blockDim.x / 32; ++i) top = max(top, stop[i]);
   const bool bad = top >= 0x7F800000u;
   const int k = bad ? 0 : min(126, 134 - (int)(top >> 23));  // the maximum to [128, 256)
   const float f = pow2i(k);
-  uint8_t* image = p.q_parts + (int64_t)v * p.q_bytes;
-#pragma unroll
-  for (int i = 0; i < kOcts; ++i) {
-    const int o = lane + 32 * i;
-    if (o >= p.boxes * 16) break;
+  if (o < p.boxes * 16) {
     float y[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = bad ? 0.f : to_f<T>(x[i].v[j]) * f;
-    uint8_t* at = image + (size_t)(o >> 4) * NS * 128 + (o & 1) * 8;
+    for (int j = 0; j < 8; ++j) y[j] = bad ? 0.f : to_f<T>(x.v[j]) * f;
+    uint8_t* at = p.q_parts + (int64_t)v * p.q_bytes + (size_t)(o >> 4) * NS * 128 + (o & 1) * 8;
 #pragma unroll
     for (int part = 0; part < QP; ++part) {
       const int n = part * R + r;
@@ -386,7 +383,7 @@ __global__ void __launch_bounds__(256) attn_tc_prep_kernel(const __grid_constant
           make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
     }
   }
-  if (lane == 0) p.coef[v * R + r] = bad ? __uint_as_float(0x7FC00000u) : p.a.scale * kLog2e * pow2i(-k);
+  if (o == 0) p.coef[v * R + r] = bad ? __uint_as_float(0x7FC00000u) : p.a.scale * kLog2e * pow2i(-k);
 }
 
 template <typename T, int RH, int QP>
@@ -416,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
   uint64_t* q_full = pv_done + 2;
   uint64_t* drain = q_full + 1;
   uint32_t* tslot = reinterpret_cast<uint32_t*>(drain + 1);
-  int* swalk = reinterpret_cast<int*>(tslot + 1);             // [3] first pair, skip, tiles
+  int* swalk = reinterpret_cast<int*>(tslot + 1);             // [3] first pair, skip, places
   int* swsum = swalk + 3;                                     // [10] tiles counted by each warp
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -440,8 +437,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     tc::mbar_init(drain, 1);
     tc::tma_prefetch(&p.map);
   }
-  // a context product may read weight parts that no row has: zeros
-  for (int i = tid; i < p.p_bufs * p.p_bytes / 16; i += kThreads) reinterpret_cast<int4*>(sp)[i] = make_int4(0, 0, 0, 0);
+  // a context product may read weight parts that no row has: zeros (warps 0 and 1 have other things to do)
+  for (int i = tid - 64; i >= 0 && i < p.p_bufs * p.p_bytes / 16; i += kThreads - 64)
+    reinterpret_cast<int4*>(sp)[i] = make_int4(0, 0, 0, 0);
   tc::fence_barrier_init();
   tc::fence_proxy_async();
   pdl_launch();
@@ -459,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     int own = 0, last = 0;
     for (int v = v0; v < v1; ++v) {
       last = pair_tiles(p, v, &len, &start);
-      own += last > 0 ? last + kStart : 0;
+      own += last > 0 ? last + p.start : 0;
     }
     __syncwarp();
     int incl = own;
@@ -483,12 +481,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     const int per = (total + p.grid - 1) / p.grid, mine = (int)blockIdx.x * per;  // < 2^31: the host bounds the tiles
     if (blockIdx.x == 0 || (mine >= at && mine < at + own)) {
       for (int v = v0; v < v1; ++v) {
-        const int n = run == 1 ? last : pair_tiles(p, v, &len, &start), places = n > 0 ? n + kStart : 0;
+        const int n = run == 1 ? last : pair_tiles(p, v, &len, &start), places = n > 0 ? n + p.start : 0;
         if (blockIdx.x == 0) p.prefix[v] = at;
         if (mine >= at && mine < at + places) {
           swalk[0] = v;
-          swalk[1] = max(0, mine - at - kStart);
-          swalk[2] = mine + per - max(mine, at + kStart);
+          swalk[1] = max(0, mine - at - p.start);
+          swalk[2] = mine + per - max(mine, at + p.start);
         }
         at += places;
       }
@@ -890,33 +888,26 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                       (row * width + l0) * elt;
         const int step = width * elt;
 #pragma unroll 1
-        for (int k = 0; k < p.boxes; k += S::EPI_BOXES) {
-          float v[S::EPI_BOXES][S::MAX_STACK][RH];
+        for (int k = 0; k < p.boxes; ++k, to += 128 * elt) {
+          float v[S::MAX_STACK][RH];
 #pragma unroll
-          for (int i = 0; i < S::EPI_BOXES; ++i)
-            if (k + i < p.boxes) {
-#pragma unroll
-              for (int g = 0; g < S::MAX_STACK; ++g)
-                if (g < p.stack) tmem_ldn<RH>(tmem + lanes + (uint32_t)((k + i) * p.np + g * R + r0), v[i][g]);
-            }
+          for (int g = 0; g < S::MAX_STACK; ++g)
+            if (g < p.stack) tmem_ldn<RH>(tmem + lanes + (uint32_t)(k * p.np + g * R + r0), v[g]);
           tmem_wait_ld();
+          const int rows = l0 + k * 128 < width ? have_rows : 0;
+          uint8_t* at = to;
 #pragma unroll
-          for (int i = 0; i < S::EPI_BOXES; ++i, to += 128 * elt) {
-            const int rows = l0 + (k + i) * 128 < width ? have_rows : 0;
-            uint8_t* at = to;
+          for (int r = 0; r < RH; ++r, at += step) {
+            const float2 f = sfac[r0 + r];
+            float x = v[0][r];
 #pragma unroll
-            for (int r = 0; r < RH; ++r, at += step) {
-              const float2 f = sfac[r0 + r];
-              float x = v[i][0][r];
-#pragma unroll
-              for (int g = 1; g < S::MAX_STACK; ++g)
-                if (g < p.stack) x += v[i][g][r];
-              // no key: the accumulator may hold a stale column, the row is zeros
-              x = f.y == 0.f ? 0.f : x * f.x * f.y;
-              if (r < rows) {
-                if (whole) *reinterpret_cast<T*>(at) = from_f<T>(x);
-                else *reinterpret_cast<float*>(at) = x;
-              }
+            for (int g = 1; g < S::MAX_STACK; ++g)
+              if (g < p.stack) x += v[g][r];
+            // no key: the accumulator may hold a stale column, the row is zeros
+            x = f.y == 0.f ? 0.f : x * f.x * f.y;
+            if (r < rows) {
+              if (whole) *reinterpret_cast<T*>(at) = from_f<T>(x);
+              else *reinterpret_cast<float*>(at) = x;
             }
           }
         }
@@ -949,30 +940,32 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 }
 
 // Joins the CTAs of a pair: weights 2^(lse_c - max), in the order of the CTAs.  A pair inside one CTA is
-// already written.  A block takes one row and 1,024 / SL columns; with many parts (a few long sequences) SL
+// already written.  A block takes one row and COLS * V * 4 columns; with many parts (a few long sequences) SL
 // groups of threads take every SL-th part each and are added up in shared memory.
 template <typename T, int SL>
-__global__ void __launch_bounds__(256) attn_tc_join_kernel(const __grid_constant__ TcParams p) {
-  constexpr int COLS = 256 / SL;  // threads along the columns, 4 columns each
+__global__ void __launch_bounds__(kJoinThreads<SL>) attn_tc_join_kernel(const __grid_constant__ TcParams p) {
+  constexpr int COLS = kJoinThreads<SL> / SL, V = SL == 1 ? 2 : 1;  // threads along the columns, V times 4 columns each
   __shared__ float4 sacc[SL > 1 ? SL : 1][COLS];
   __shared__ float slse[SL > 1 ? kMaxGrid : 1], sstat[SL > 1 ? 8 + SL : 1];
   const int v = blockIdx.x / p.rows_tile, r = blockIdx.x - v * p.rows_tile;
   const int b = v / p.row_tiles, row0 = (v - b * p.row_tiles) * p.rows_tile, width = p.a.cache.width;
   const int pairs = p.a.batch * p.row_tiles;
+  const int col = threadIdx.x % COLS, grp = threadIdx.x / COLS, l0 = (blockIdx.y * COLS * V + col) * 4;
+  const float* lse = p.part_lse + (int64_t)v * p.rows_tile + r;
+  const float* po = p.part_o + ((int64_t)v * p.rows_tile + r) * width;
   pdl_wait();
   if (row0 + r >= p.rows) return;
   const int at = p.prefix[v], places = p.prefix[v + 1] - at, per = p.prefix[pairs + 1];
-  const int n = places - kStart;  // tiles, if any
-  const int c0 = n > 0 ? (at + kStart) / per : 0, c1 = n > 0 ? (at + places - 1) / per : -1;
+  const int n = places - p.start;  // tiles, if any
+  const int c0 = n > 0 ? (at + p.start) / per : 0, c1 = n > 0 ? (at + places - 1) / per : -1;
   if (n > 0 && c0 == c1) return;
-  const int col = threadIdx.x % COLS, grp = threadIdx.x / COLS, l = (blockIdx.y * COLS + col) * 4;
-  const float* lse = p.part_lse + (int64_t)v * p.rows_tile + r;
-  const float* po = p.part_o + ((int64_t)v * p.rows_tile + r) * width + (l < width ? l : 0);
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 acc[V];
   float m = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < V; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
   if constexpr (SL > 1) {  // all log-sums at once
     const int parts = c1 - c0 + 1;  // <= kMaxGrid
-    for (int i = threadIdx.x; i < parts; i += 256) {
+    for (int i = threadIdx.x; i < parts; i += kJoinThreads<SL>) {
       slse[i] = lse[(int64_t)(c0 + i) * p.rows_tile];
       m = fmaxf(m, slse[i]);
     }
@@ -981,64 +974,79 @@ __global__ void __launch_bounds__(256) attn_tc_join_kernel(const __grid_constant
     __syncthreads();
     m = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, sstat[i]);
+    for (int i = 0; i < kJoinThreads<SL> / 32; ++i) m = fmaxf(m, sstat[i]);
   }
   // four parts in flight; without the log-sums at hand the weights follow a running maximum
   for (int c = c0 + grp; c <= c1; c += 4 * SL) {
     float f[4];
-    float4 x[4];
+    float4 x[4][V];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int ci = c + i * SL;
       const bool on = ci <= c1;
       f[i] = !on ? -INFINITY : SL > 1 ? slse[ci - c0] : lse[(int64_t)ci * p.rows_tile];
-      x[i] = on ? *reinterpret_cast<const float4*>(po + (int64_t)ci * p.rows_tile * width) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const int l = l0 + k * COLS * 4;
+        x[i][k] = on && l < width ? *reinterpret_cast<const float4*>(po + (int64_t)ci * p.rows_tile * width + l)
+                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
     }
     if constexpr (SL == 1) {
       const float to = fmaxf(fmaxf(m, fmaxf(f[0], f[1])), fmaxf(f[2], f[3]));
       const float g = m == to || to == -INFINITY ? 1.f : exp2f(m - to);
       m = to;
       sum *= g;
-      acc.x *= g;
-      acc.y *= g;
-      acc.z *= g;
-      acc.w *= g;
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        acc[k].x *= g;
+        acc[k].y *= g;
+        acc[k].z *= g;
+        acc[k].w *= g;
+      }
     }
     const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float e = exp2f(f[i] - base);  // 0 for a part that is not there
       sum += e;
-      acc.x += e * x[i].x;
-      acc.y += e * x[i].y;
-      acc.z += e * x[i].z;
-      acc.w += e * x[i].w;
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        acc[k].x += e * x[i][k].x;
+        acc[k].y += e * x[i][k].y;
+        acc[k].z += e * x[i][k].z;
+        acc[k].w += e * x[i][k].w;
+      }
     }
   }
   if constexpr (SL > 1) {
-    sacc[grp][col] = acc;
+    sacc[grp][col] = acc[0];
     if (col == 0) sstat[8 + grp] = sum;
     __syncthreads();
     if (grp != 0) return;
     for (int g = 1; g < SL; ++g) {
       const float4 x = sacc[g][col];
-      acc.x += x.x;
-      acc.y += x.y;
-      acc.z += x.z;
-      acc.w += x.w;
+      acc[0].x += x.x;
+      acc[0].y += x.y;
+      acc[0].z += x.z;
+      acc[0].w += x.w;
       sum += sstat[8 + g];
     }
   }
-  if (l >= width) return;
   const float inv = sum != 0.f ? 1.f / sum : 0.f;
-  T* out = static_cast<T*>(p.a.out) + ((int64_t)b * p.rows + row0 + r) * width + l;
-  const float o[4] = {acc.x, acc.y, acc.z, acc.w};
-  struct alignas(4 * sizeof(T)) Four {
-    T t[4];
-  } four;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) four.t[i] = from_f<T>(inv == 0.f ? 0.f : o[i] * inv);
-  *reinterpret_cast<Four*>(out) = four;
+  for (int k = 0; k < V; ++k) {
+    const int l = l0 + k * COLS * 4;
+    if (l >= width) continue;
+    T* out = static_cast<T*>(p.a.out) + ((int64_t)b * p.rows + row0 + r) * width + l;
+    const float o[4] = {acc[k].x, acc[k].y, acc[k].z, acc[k].w};
+    struct alignas(4 * sizeof(T)) Four {
+      T t[4];
+    } four;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) four.t[i] = from_f<T>(inv == 0.f ? 0.f : o[i] * inv);
+    *reinterpret_cast<Four*>(out) = four;
+  }
 }
 
 // Weight parts on N cost accumulator columns, parts along K cost a pass over the tile (36 + N / 5 clocks
@@ -1216,7 +1224,7 @@ cudaError_t launch(const TcParams& p, const Plan& pl, cudaStream_t s) {
   cudaError_t e = ensure_dynamic_smem(kern, (int)pl.smem);
   if (e != cudaSuccess) return e;
   const int pairs = p.a.batch * p.row_tiles;
-  e = launch_dependent(attn_tc_prep_kernel<T, QP>, dim3((pairs * p.rows_tile + 7) / 8), 256, 0, s, p);
+  e = launch_dependent(attn_tc_prep_kernel<T, QP>, dim3(pairs * p.rows_tile), (p.boxes * 16 + 31) / 32 * 32, 0, s, p);
   if (e != cudaSuccess) return e;
   if ((e = launch_dependent(kern, dim3(pl.grid), kThreads, pl.smem, s, p)) != cudaSuccess || pl.direct) return e;
   const unsigned rows = (unsigned)(pairs * p.rows_tile);
@@ -1224,7 +1232,7 @@ cudaError_t launch(const TcParams& p, const Plan& pl, cudaStream_t s) {
   if (pl.grid >= 32 * pairs)  // many parts of few pairs
     return launch_dependent(attn_tc_join_kernel<T, 8>, dim3(rows, (width + 127) / 128), 256, 0, s, p);
   if (pl.grid >= 6 * pairs) return launch_dependent(attn_tc_join_kernel<T, 2>, dim3(rows, (width + 511) / 512), 256, 0, s, p);
-  return launch_dependent(attn_tc_join_kernel<T, 1>, dim3(rows, (width + 1023) / 1024), 256, 0, s, p);
+  return launch_dependent(attn_tc_join_kernel<T, 1>, dim3(rows, (width + 1023) / 1024), kJoinThreads<1>, 0, s, p);
 }
 
 template <typename T, int QP>
@@ -1243,7 +1251,7 @@ cudaError_t launch_rh(const TcParams& p, const Plan& pl, cudaStream_t s) {
 // Code rows that TMA can address: 16-byte base and strides.
 bool mla_attn_tc_supported(int dtype, const MlaCacheAttnArgs& a) {
   if (dtype < 0 || dtype > 2) return false;
-  if (a.cache.width % 16 || a.cache.width < 64 || a.cache.width > 256 * kOcts || a.cache.slots > (1 << 30)) return false;
+  if (a.cache.width % 16 || a.cache.width < 64 || a.cache.width > 8 * kPrepThreads || a.cache.slots > (1 << 30)) return false;
   if ((reinterpret_cast<uintptr_t>(a.cache.codes) & 15) || (a.batch > 1 && a.cache.code_b % 16)) return false;
   if (a.cache.slots > 1 && (a.cache.code_t % 16 || a.cache.code_t < a.cache.width)) return false;
   Plan pl;
@@ -1294,6 +1302,7 @@ cudaError_t mla_attn_tc(int dtype, const MlaCacheAttnArgs& a, cudaStream_t s) {
   p.p_bufs = pl.p_bufs;
   p.q_bytes = pl.boxes * pl.ns * 128;
   p.grid = pl.grid;
+  p.start = (a.cache.slots + kTile - 1) / kTile * a.batch * pl.row_tiles <= pl.grid ? 0 : kStart;
   p.fetch = kFetch;
   p.direct = pl.direct ? 1 : 0;
   p.tmem = pl.tmem;
