@@ -8,6 +8,10 @@
 // element.  One warp owns one token row.  The writer holds its row in registers between the maximum
 // and the rounding, so x crosses HBM once; the maximum runs on the magnitudes' bit patterns, which
 // order like the values and put infinities and NaN on top, two 16-bit elements per instruction.
+//
+// The copy rate bounds both: 64 x 4,096 rows of 1,536 in bf16 (1.21 GB) are written in 175 us (6.9 TB/s) and
+// read in 185 us (6.5 TB/s; a measured plain copy: 6.55).  One decode step's 64 rows are 4.5 us of a caller's
+// time, 1.5 to 2.2 on the GPU: the launch.
 #include <type_traits>
 
 #include "mla_cache.cuh"
@@ -72,7 +76,7 @@ struct Oct<float> {
   static KIMI_D uint32_t bits(uint32_t t) { return t; }
 };
 
-// Sequence and token of a row; the launchers bound the rows by 2^31 (a 64-bit division is ten times a 32-bit one).
+// Sequence and token of a row; the launchers bound the rows by 2^31, so the division needs 32 bits only.
 KIMI_D bool row_of(int64_t tokens, int batch, int* b, int64_t* j) {
   const uint32_t row = blockIdx.x * kRowWarps + (threadIdx.x >> 5), t = (uint32_t)tokens;
   const uint32_t q = row / t;

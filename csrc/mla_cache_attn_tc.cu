@@ -17,12 +17,11 @@
 // Splitting into 8-bit parts keeps the query type's accuracy.  A query row is scaled by a power of two to
 // [128, 256) and written as q = q0 + q1 / 32 + q2 / 1024 + .. in e4m3, each part the rounding of what the
 // one before left (5 bits a part): two parts hold every bf16, three every fp16, five every fp32 but for
-// what lies more than 2^-18, 2^-27, 2^-38 below the row's maximum.  The parts sit side by side on N (A is read once) and are added in fp32.  The weights
-// v = 2^(s + log2(scale_t) - ref) <= 2^15 are split into e5m2 parts (3 + 4 + 4 + .. bits) along K, all
-// accumulating into the same columns: three for bf16 outputs (11 bits), four for fp16 (14), six for fp32
-// (22).  e5m2
-// because of its range: the parts of a weight 2^-18 below the row's reference are still whole, where
-// e4m3's step of 2^-9 would cut what many small weights add up to.
+// what lies more than 2^-18, 2^-27, 2^-38 below the row's maximum.  The parts sit side by side on N (A is
+// read once) and are added in fp32.  The weights v = 2^(s + log2(scale_t) - ref) <= 2^15 are split into
+// e5m2 parts (3 + 4 + 4 + .. bits), all added up in fp32: three for bf16 outputs (11 bits), four for fp16
+// (14), six for fp32 (22).  e5m2 because of its range: it ends at 2^-16, so all 11 bits of a weight are there
+// down to 2^-20 of the largest possible, where e4m3's step of 2^-9 would cut what many small weights add up to.
 //
 // The softmax reference of a row is a power of two that only moves when some weight would pass 2^15
 // (then the row's accumulator columns are rescaled in TMEM, exactly); the sums use the scores alone
@@ -37,6 +36,14 @@
 // query parts; the attention, each CTA of which finds its own range of the list; the join.  The query parts are written as
 // the image of their shared-memory tile, so that a CTA brings in the next sequence's queries with one
 // bulk copy while it still works on the last tile of this one.
+//
+// What bounds it.  One product reads its tile from shared memory once per run of weight parts, at 128 bytes a clock:
+// with 24 rows of width 1536 a tile of 96 KB is written once, read once (with 72 KB of query parts) for the scores and
+// three times (with 24 KB of weights each) for the context, 4,980 clocks of shared memory in a measured 6,260; the rest
+// is scores -> weights -> context one behind the other, since 72 KB of query parts leave a ring of one and a half tiles.
+// With 12 rows it is 3,770 in 4,730, with 3 rows the memory: 64 x 4,608 tokens of width 1536 (453 MB) take 92 - 96 us
+// for 3 heads (4.8 TB/s, 73 % of the measured copy), 158 for 24.  Under this load the GPU runs at its power limit.
+// Short calls are three launches and one tile's latency: 12.8 us for one sequence of 257 tokens on the GPU alone.
 //
 // Roles of an attention CTA (10 warps): warp 0 loads, warp 1 issues the MMAs, warps 2-9 are two groups
 // of four that share the rows: scores -> weights, rescaling and the epilogue.
@@ -60,8 +67,12 @@ constexpr int kTile = 64;                  // tokens of a tile
 constexpr int kBox = kTile * 128;          // bytes of a box
 constexpr int kThreads = 320;
 constexpr int kMaxStages = 32;             // of the ring
-constexpr int kFetch = 1;                  // tiles ahead that are brought into L2
-constexpr int kMaxGroup = 8;               // boxes of a stage
+// Tiles ahead that are brought into L2 (the ring holds one and a half at width 1536); 0 / 1, 64 x 4,608, width 1536:
+// 24 heads 150.7 / 142.7 us, 12 heads 122.3 / 108.8, 3 heads 87.3 / 83.6.
+constexpr int kFetch = 1;
+// Boxes of a ring stage, at most: a wide stage reads long pieces of each cached row together.  3 / 4 / 8 boxes: 64 x 6,144,
+// 16 heads, width 1024 103.0 / 92.9 / 86.1 us; 64 x 4,096, 10 heads, width 640 (five boxes) 56.8 / 56.8 / 49.5.
+constexpr int kMaxGroup = 8;
 constexpr int kSmemMax = 227 * 1024;
 constexpr int kMaxGrid = 256;              // CTAs of the attention kernel
 template <int SL>
@@ -69,10 +80,13 @@ constexpr int kJoinThreads = SL == 1 ? 128 : 256;
 constexpr int kPrepThreads = 256;          // 8 elements of a query row each: widths up to 2,048
 constexpr int kMisaligned = 9;             // status: shared memory off a 1,024-byte boundary
 constexpr float kTop = 15.f;               // a weight may reach 2^kTop
-// a new reference leaves this many bits: fewer moves of the accumulators against a lower floor of the weights
-// (2^-26 of the largest; 2^-31 for fp32 results)
+// A new reference leaves the row's largest weight at 2^(kTop - kRoom): each bit of room saves moves of the
+// accumulators (a stall of the CTA) and raises the floor of the weights, 2^(kRoom - 32) of the largest, where
+// e5m2 ends.  As many bits as keep weights down to about 2^-15 of the largest within one unit of the output's
+// type: bf16 9, fp16 6; fp32 1.  bf16 with 6 / 9, random queries and cache of 64 x 4,608, width 1536: 24 heads
+// 168 / 158 us, 12 heads of ragged lengths 83.1 / 76.7.
 template <int QP>
-constexpr float kRoom = QP == 5 ? 1.f : 6.f;
+constexpr float kRoom = QP == 2 ? 9.f : QP == 3 ? 6.f : 1.f;
 constexpr float kNoRef = -3e38f;            // finite: a score of -inf weighs nothing against it
 constexpr float kSumRoom = 40.f;           // the sums' reference may lag by this many bits
 
@@ -295,7 +309,8 @@ KIMI_D int pair_tiles(const TcParams& p, int v, int64_t* len_out, int64_t* start
 
 // The list of all pairs' tiles is cut into equal ranges, one per CTA.  Starting a pair costs a CTA about as
 // much as kStart tiles (an epilogue, an empty pipeline), so each pair with tiles has kStart places in front;
-// none where every tile can have its own CTA.
+// none where every tile can have its own CTA.  0 / 2 / 4, 64 x 4,608, width 1536: 24 heads 147 / 143 / 142 us,
+// 12 heads 112 / 109 / 112, 3 heads 85.4 / 83.8 / 85.4.
 constexpr int kStart = 2;
 
 // This CTA's share of the list, walked pair by pair (every role walks it on its own).
@@ -1053,7 +1068,9 @@ __global__ void __launch_bounds__(kJoinThreads<SL>) attn_tc_join_kernel(const __
 }
 
 // Weight parts on N cost accumulator columns, parts along K cost a pass over the tile (36 + N / 5 clocks
-// per 32 tokens x 128 latents as measured, whatever N holds): as many on N as make the passes cheapest.
+// per 32 tokens x 128 latents as measured, whatever N holds): as many on N as make the passes cheapest.  One
+// part on N / as chosen: 64 x 4,608, width 1536 12 heads 121.3 / 108.8 us (two on N), 3 heads 113.2 / 83.8 (three);
+// 64 x 4,096, 10 heads, width 640 59.3 / 49.7 (three).
 template <int RH, int QP>
 bool fit(int boxes, Plan* pl) {
   using S = Shape<RH, QP>;
@@ -1066,9 +1083,9 @@ bool fit(int boxes, Plan* pl) {
     const int cost = runs * (36 * 5 + np);
     if (found && cost >= best && bufs <= pl->s_bufs) continue;
     const int p_bytes = np * 128 * ((runs + 1) / 2);
-    // Stages as wide as the ring allows with a tile in it and more to load: a wide stage reads long pieces of
-    // each cached row together.  Where the ring holds less than two tiles, a tile's weights are written only
-    // once the tile before has left the ring: one weight buffer then costs no time and widens the ring.
+    // Stages as wide as the ring allows with a tile in it and more to load.  Where the ring holds less than two
+    // tiles, a tile's weights are written only once the tile before has left the ring: one weight buffer then
+    // costs no time and widens the ring (24 heads, width 1536: 143 us, 152 with two; 12 heads the same).
     int tile_stages = 0, group = 0, stages = 0, p_bufs = 2;
     size_t fixed = 0;
     for (; p_bufs >= 1; --p_bufs) {
@@ -1261,7 +1278,8 @@ cudaError_t launch_rh(const TcParams& p, const Plan& pl, cudaStream_t s) {
 // Code rows that TMA can address: 16-byte base and strides.
 bool mla_attn_tc_supported(int dtype, const MlaCacheAttnArgs& a) {
   if (dtype < 0 || dtype > 2) return false;
-  if (a.cache.width % 16 || a.cache.width < 64 || a.cache.width > 8 * kPrepThreads || a.cache.slots > (1 << 30)) return false;
+  if (a.cache.width % 16 || a.cache.width < 64 || a.cache.width > 8 * kPrepThreads) return false;
+  if (a.cache.slots > (1 << 30)) return false;
   if ((reinterpret_cast<uintptr_t>(a.cache.codes) & 15) || (a.batch > 1 && a.cache.code_b % 16)) return false;
   if (a.cache.slots > 1 && (a.cache.code_t % 16 || a.cache.code_t < a.cache.width)) return false;
   Plan pl;

@@ -524,8 +524,11 @@ def absorbed_latent_decode(query, latent_cache, cache_mask, key_up_weight, value
 
 # Query tokens per row up to which a quantized cache is attended in the latent space.  Per cached token the
 # absorbed form costs 4 H L flops for every query token, rebuilding K and V 2 L H (Dq + Dv) once and
-# 2 H (Dq + Dv) per query token besides the traffic of K and V (and of the scores) through memory.
-ABSORBED_QUERY_LIMIT = 16
+# 2 H (Dq + Dv) per query token besides the traffic of K and V (and of the scores) through memory.  A layer's
+# forward in us, absorbed / rebuilt, at 16, 64, 128 and 256 query tokens: 64 sequences of 2,048, 10 heads, width 640
+# 603 / 2408, 1016 / 2624, 1672 / 2824, 2974 / 2793; 16 of 4,096, 24 heads, width 1536 901 / 3148, 2177 / 3310,
+# 3927 / 3436, 7472 / 3065.
+ABSORBED_QUERY_LIMIT = 64
 
 
 def absorbed_quantized_attention(query, cache: QuantizedMLACache, key_up_weight, value_up_weight, num_heads, *,

@@ -126,13 +126,13 @@ def test_refusals():
 
 
 # ------------------------------------------------------------------------------------------ the layer
-@pytest.mark.parametrize("tokens", [1, 3, ABSORBED_QUERY_LIMIT, ABSORBED_QUERY_LIMIT + 5])
+@pytest.mark.parametrize("tokens", [1, 3, 16, 21, ABSORBED_QUERY_LIMIT, ABSORBED_QUERY_LIMIT + 5])
 @pytest.mark.parametrize("ragged", [False, True])
 def test_layer_on_the_quantised_cache(tokens, ragged):
     torch.manual_seed(3)
     cfg = GatedMLAConfig(d_model=24, num_heads=3, q_head_dim=8, v_head_dim=8, kv_latent_dim=16)
     layer = GatedMLA(cfg).double().eval()
-    b, prompt, slots = 3, 7, 40
+    b, prompt, slots = 3, 7, 40 if tokens <= 21 else tokens + 19
     mask0 = torch.ones(b, prompt, dtype=torch.bool)
     mask0[1, 4:] = False
     with torch.no_grad():

@@ -451,6 +451,29 @@ def test_layer_against_its_plain_form(cuda, tokens, dtype, monkeypatch):
     assert err <= (2.0 ** -6 if dtype == torch.bfloat16 else 2.0 ** -11), err
 
 
+@pytest.mark.parametrize("limit", [0, 64])
+def test_layer_attends_or_rebuilds(cuda, limit, monkeypatch):
+    """The layer's two forms on a quantised cache, in the latent space and over rebuilt keys and values, at one length:
+    each within a few roundings of the PyTorch form of the same layer in fp32."""
+    from kimi_k3_b200.models import mla
+    torch.manual_seed(8)
+    layer = mla.GatedMLA(mla.GatedMLAConfig(d_model=640, num_heads=10, q_head_dim=64, v_head_dim=64,
+                                            kv_latent_dim=640)).to(cuda).eval()
+    b, prompt, tokens = 2, 90, 30
+    x0, x = torch.randn(b, prompt, 640, device=cuda), torch.randn(b, tokens, 640, device=cuda)
+    mask0 = torch.arange(prompt, device=cuda)[None, :] < torch.tensor([90, 41], device=cuda)[:, None]
+    mask = torch.arange(tokens, device=cuda)[None, :] < torch.tensor([30, 11], device=cuda)[:, None]
+    outs = []
+    with torch.no_grad():
+        first = mla.QuantizedMLACache.from_cache(layer(x0, mask0, use_cache=True).cache, 130)
+        for kernels, n in (("1", limit), ("0", 0)):
+            monkeypatch.setenv("KIMI_K3_KERNELS", kernels)
+            monkeypatch.setattr(mla, "ABSORBED_QUERY_LIMIT", n)
+            outs.append(layer(x, mask, cache=first.clone(), use_cache=True).hidden_states)
+    err = (outs[0] - outs[1]).abs().max().item() / outs[1].abs().max().item()
+    assert err <= 2.0 ** -11, err
+
+
 def test_graph_decoder_on_a_quantised_cache(cuda):
     from kimi_k3_b200.infer import GenerationConfig, GraphDecoder
     from kimi_k3_b200.models.mla import QuantizedMLACache
