@@ -11,7 +11,8 @@
 //
 // The copy rate bounds both: 64 x 4,096 rows of 1,536 in bf16 (1.21 GB) are written in 175 us (6.9 TB/s) and
 // read in 185 us (6.5 TB/s; a measured plain copy: 6.55).  One decode step's 64 rows are 4.5 us of a caller's
-// time, 1.5 to 2.2 on the GPU: the launch.
+// time, 1.5 to 2.2 on the GPU: the launch.  Splitting a row's number by a 32-bit division saved the small calls
+// nothing and cost the large write 8 % (189 us).
 #include <type_traits>
 
 #include "mla_cache.cuh"
@@ -76,15 +77,6 @@ struct Oct<float> {
   static KIMI_D uint32_t bits(uint32_t t) { return t; }
 };
 
-// Sequence and token of a row; the launchers bound the rows by 2^31, so the division needs 32 bits only.
-KIMI_D bool row_of(int64_t tokens, int batch, int* b, int64_t* j) {
-  const uint32_t row = blockIdx.x * kRowWarps + (threadIdx.x >> 5), t = (uint32_t)tokens;
-  const uint32_t q = row / t;
-  *b = (int)q;
-  *j = row - q * t;
-  return q < (uint32_t)batch;
-}
-
 // Slot of token j of sequence b, or -1.
 KIMI_D int64_t write_slot(const MlaCacheWriteArgs& a, int b, int64_t j) {
   if (a.counts.p && j >= get(a.counts, b)) return -1;
@@ -96,9 +88,10 @@ KIMI_D int64_t write_slot(const MlaCacheWriteArgs& a, int b, int64_t j) {
 template <typename T, int OCTS>
 __global__ void __launch_bounds__(kRowWarps * 32) write_kernel(const __grid_constant__ MlaCacheWriteArgs a) {
   const int lane = threadIdx.x & 31;
-  int b;
-  int64_t j;
-  if (!row_of(a.tokens, a.batch, &b, &j)) return;
+  const int64_t row = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
+  if (row >= (int64_t)a.batch * a.tokens) return;
+  const int b = (int)(row / a.tokens);
+  const int64_t j = row - (int64_t)b * a.tokens;
   const int64_t slot = write_slot(a, b, j);
   if (slot < 0) return;
   const T* x = static_cast<const T*>(a.x) + b * a.x_b + j * a.x_t;
@@ -137,9 +130,10 @@ __global__ void __launch_bounds__(kRowWarps * 32) write_kernel(const __grid_cons
 template <typename T>
 __global__ void __launch_bounds__(kRowWarps * 32) write_any_kernel(const __grid_constant__ MlaCacheWriteArgs a) {
   const int lane = threadIdx.x & 31;
-  int b;
-  int64_t j;
-  if (!row_of(a.tokens, a.batch, &b, &j)) return;
+  const int64_t row = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
+  if (row >= (int64_t)a.batch * a.tokens) return;
+  const int b = (int)(row / a.tokens);
+  const int64_t j = row - (int64_t)b * a.tokens;
   const int64_t slot = write_slot(a, b, j);
   if (slot < 0) return;
   const T* x = static_cast<const T*>(a.x) + b * a.x_b + j * a.x_t;
@@ -158,13 +152,14 @@ __global__ void __launch_bounds__(kRowWarps * 32) write_any_kernel(const __grid_
 template <typename T, bool OCT>
 __global__ void __launch_bounds__(kRowWarps * 32) read_kernel(const __grid_constant__ MlaCacheReadArgs a) {
   const int lane = threadIdx.x & 31;
-  int b;
-  int64_t j;
-  if (!row_of(a.tokens, a.batch, &b, &j)) return;
+  const int64_t row = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
+  if (row >= (int64_t)a.batch * a.tokens) return;
+  const int b = (int)(row / a.tokens);
+  const int64_t j = row - (int64_t)b * a.tokens;
   const bool live = !a.lengths.p || j < get(a.lengths, b);
   const uint8_t* c = a.cache.codes + b * a.cache.code_b + j * a.cache.code_t;
   const float s = live ? a.cache.scales[b * a.cache.scale_b + j * a.cache.scale_t] : 0.f;
-  T* y = static_cast<T*>(a.out) + ((int64_t)b * a.tokens + j) * a.cache.width;
+  T* y = static_cast<T*>(a.out) + row * a.cache.width;
   if constexpr (OCT) {
     const int octs = a.cache.width >> 3;
 #pragma unroll 4
@@ -198,7 +193,7 @@ bool aligned(const void* p, int64_t to) { return (reinterpret_cast<uintptr_t>(p)
 template <typename T>
 cudaError_t launch_write(const MlaCacheWriteArgs& a, cudaStream_t s) {
   const int64_t rows = (int64_t)a.batch * a.tokens, grid = (rows + kRowWarps - 1) / kRowWarps;
-  if (rows > 0x7FFFFFF0) return cudaErrorInvalidValue;
+  if (grid > 0x7FFFFFFF) return cudaErrorInvalidValue;
   const int64_t eb = a.x_b * (int64_t)sizeof(T), et = a.x_t * (int64_t)sizeof(T);
   const bool oct = a.cache.width % 8 == 0 && aligned(a.x, 16) && eb % 16 == 0 && et % 16 == 0 &&
                    aligned(a.cache.codes, 8) && a.cache.code_b % 8 == 0 && a.cache.code_t % 8 == 0;
@@ -221,7 +216,7 @@ cudaError_t launch_write(const MlaCacheWriteArgs& a, cudaStream_t s) {
 template <typename T>
 cudaError_t launch_read(const MlaCacheReadArgs& a, cudaStream_t s) {
   const int64_t rows = (int64_t)a.batch * a.tokens, grid = (rows + kRowWarps - 1) / kRowWarps;
-  if (rows > 0x7FFFFFF0) return cudaErrorInvalidValue;
+  if (grid > 0x7FFFFFFF) return cudaErrorInvalidValue;
   const bool oct = a.cache.width % 8 == 0 && aligned(a.cache.codes, 8) && a.cache.code_b % 8 == 0 &&
                    a.cache.code_t % 8 == 0 && aligned(a.out, 16);
   if (oct) read_kernel<T, true><<<(unsigned)grid, kRowWarps * 32, 0, s>>>(a);
