@@ -39,9 +39,10 @@
 //
 // What bounds it.  One product reads its tile from shared memory once per run of weight parts, at 128 bytes a clock:
 // with 24 rows of width 1536 a tile of 96 KB is written once, read once (with 72 KB of query parts) for the scores and
-// three times (with 24 KB of weights each) for the context, 4,980 clocks of shared memory in a measured 6,260; the rest
-// is scores -> weights -> context one behind the other, since 72 KB of query parts leave a ring of one and a half tiles.
-// With 12 rows it is 3,770 in 4,730, with 3 rows the memory: 64 x 4,608 tokens of width 1536 (453 MB) take 92 - 96 us
+// three times (with 24 KB of weights each) for the context: by that count 4,980 clocks of a measured 6,260 (the counters
+// show 57 % of the shared-memory and L1 throughput over the whole kernel); the rest is scores -> weights -> context one
+// behind the other, since 72 KB of query parts leave a ring of one and a half tiles.
+// With 12 rows the count is 3,770 of 4,730, with 3 rows the memory bounds: 64 x 4,608 tokens of width 1536 (453 MB) take 92 - 96 us
 // for 3 heads (4.8 TB/s, 73 % of the measured copy), 158 for 24.  Under this load the GPU runs at its power limit.
 // Short calls are three launches and one tile's latency: 12.8 us for one sequence of 257 tokens on the GPU alone.
 //
@@ -67,8 +68,8 @@ constexpr int kTile = 64;                  // tokens of a tile
 constexpr int kBox = kTile * 128;          // bytes of a box
 constexpr int kThreads = 320;
 constexpr int kMaxStages = 32;             // of the ring
-// Tiles ahead that are brought into L2 (the ring holds one and a half at width 1536); 0 / 1, 64 x 4,608, width 1536:
-// 24 heads 150.7 / 142.7 us, 12 heads 122.3 / 108.8, 3 heads 87.3 / 83.6.
+// Tiles ahead that are brought into L2 (the ring holds one and a half at width 1536).  0 / 1, back to back, 64 x 4,608,
+// width 1536: 24 heads 150.7 / 142.7 us, 12 heads 122.3 / 108.8, 3 heads 87.3 / 83.6.
 constexpr int kFetch = 1;
 // Boxes of a ring stage, at most: a wide stage reads long pieces of each cached row together.  3 / 4 / 8 boxes: 64 x 6,144,
 // 16 heads, width 1024 103.0 / 92.9 / 86.1 us; 64 x 4,096, 10 heads, width 640 (five boxes) 56.8 / 56.8 / 49.5.
