@@ -905,6 +905,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         const int step = width * elt;
 #pragma unroll 1
         for (int k = 0; k < p.boxes; ++k, to += 128 * elt) {
+          __syncwarp();  // the box before may have been the end of some lanes' columns
           float v[S::MAX_STACK][RH];
 #pragma unroll
           for (int g = 0; g < S::MAX_STACK; ++g)
