@@ -687,20 +687,23 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     bool ok = true;
     uint32_t n_tile = 0;
     int stage = 0;  // first stage of the tile
-    auto wait = [&](uint64_t* bar, uint32_t use, int code) {  // the warp is converged again behind it
-      ok = ok && tc::mbar_wait(bar, use & 1, p.status, code);
-      __syncwarp();
+    auto wait = [&](uint64_t* bar, uint32_t use, int code) {  // the warp is converged again behind it, and agrees
+      ok = __all_sync(0xffffffffu, ok && tc::mbar_wait(bar, use & 1, p.status, code));
       tc::tc_fence_after();
     };
+    // One copy at a time: the next is issued behind a wait that shows the one before to be read.
+    uint32_t n_q = 0;  // warp 2: copies issued
     auto load_q = [&](int v) {
       tc::mbar_arrive_expect_tx(q_full, p.q_bytes);
       bulk_load(sq, p.q_parts + (int64_t)v * p.q_bytes, p.q_bytes, q_full);
     };
     pdl_wait();  // the query parts are there
     bool have = w.next(p, pairs);
-    if (have && warp == 2 && elect_one()) load_q(w.v);
+    if (have && warp == 2) {
+      if (elect_one()) load_q(w.v);
+      ++n_q;
+    }
     __syncwarp();
-    uint32_t seg = 0;
     while (have) {
       const int b = w.v / p.row_tiles, row0 = (w.v - b * p.row_tiles) * p.rows_tile;
       const int nrow = min(p.rows_tile, p.rows - row0);
@@ -730,7 +733,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         const uint32_t buf = p.s_bufs == 2 ? n_tile & 1 : 0, pb = n_tile & 1;
         wait(&s_full[buf], p.s_bufs == 2 ? n_tile >> 1 : n_tile, tc::kTimeoutTmemFull);
         // this segment's score products are done: the next one's queries may come in
-        if (t + 1 == w.t1 && more && warp == 2 && elect_one()) load_q(nx.v);
+        if (t + 1 == w.t1 && more && warp == 2 && ok) {
+          if (elect_one()) load_q(nx.v);
+          ++n_q;
+        }
         __syncwarp();
         float s[HR];
         {
@@ -933,7 +939,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       group_sync(bar_id);  // references and sums of the group are rewritten next
       w = nx;
       have = more;
-      ++seg;
     }
     if (p.direct && swalk[2] == 0) {  // a pair without a key
       const int b = blockIdx.x / p.row_tiles, row0 = (blockIdx.x - b * p.row_tiles) * p.rows_tile;
@@ -942,8 +947,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       for (int64_t i = tid - 64; i < n; i += 256) out[i] = from_f<T>(0.f);
     }
     // a query copy that nobody waited for (a wait failed before its turn) lands before the CTA ends
-    if (seg > 0 && warp == 2 && elect_one())
-      tc::mbar_wait_local(q_full, (seg - 1) & 1, p.status, tc::kTimeoutDrain, tc::kDrainNs);
+    if (n_q > 0 && warp == 2 && elect_one())
+      tc::mbar_wait_local(q_full, (n_q - 1) & 1, p.status, tc::kTimeoutDrain, tc::kDrainNs);
     __syncwarp();
   }
   tc::tc_fence_before();
