@@ -36,12 +36,12 @@ size_t generic_smem(int width) {
          3 * kRows * sizeof(float);
 }
 
-// fp32 arithmetic on any width and alignment: the form for what TMA cannot address (widths, strides or
-// a base that are no multiples of 16 bytes; widths under 64).  A warp scores 4 tokens x 8 rows
+// fp32 arithmetic on any width and alignment: the form for fp32 queries and for what TMA cannot address (widths, strides
+// or a base that are no multiples of 16 bytes; widths under 64).  A warp scores 4 tokens x 8 rows
 // per pass over the latent axis (a lane holds four adjacent columns: 128 FMAs per 12 shared-memory
 // loads); in the context phase a thread owns four adjacent columns of up to CP groups of 1,024.  The FMA
 // pipes bound it: 16 x 2,048 tokens, 12 heads take 302 us at width 1,544, where TMA cannot address the rows,
-// and 32 us on the tensor cores at width 1,552.
+// and 32 us on the tensor cores at width 1,552.  fp32 queries: 4 x up to 1,000 tokens, 10 heads, width 640 35.9 us.
 template <typename T, int CP>
 __global__ void __launch_bounds__(kThreads) attn_any_kernel(const __grid_constant__ MlaCacheAttnArgs a) {
   extern __shared__ __align__(16) unsigned char any_smem[];

@@ -16,12 +16,16 @@
 //
 // Splitting into 8-bit parts keeps the query type's accuracy.  A query row is scaled by a power of two to
 // [128, 256) and written as q = q0 + q1 / 32 + q2 / 1024 + .. in e4m3, each part the rounding of what the
-// one before left (5 bits a part): two parts hold every bf16, three every fp16, five every fp32 but for
-// what lies more than 2^-18, 2^-27, 2^-38 below the row's maximum.  The parts sit side by side on N (A is
+// one before left (5 bits a part): two parts hold every bf16 and three every fp16 but for what lies more than
+// 2^-18, 2^-27 below the row's maximum.  The parts sit side by side on N (A is
 // read once) and are added in fp32.  The weights v = 2^(s + log2(scale_t) - ref) <= 2^15 are split into
 // e5m2 parts (3 + 4 + 4 + .. bits), all added up in fp32: three for bf16 outputs (11 bits), four for fp16
-// (14), six for fp32 (22).  e5m2 because of its range: it ends at 2^-16, so all 11 bits of a weight are there
+// (14).  e5m2 because of its range: it ends at 2^-16, so all 11 bits of a weight are there
 // down to 2^-20 of the largest possible, where e4m3's step of 2^-9 would cut what many small weights add up to.
+//
+// fp32 queries do not come here.  With more parts (five of the query, six of a weight) the operands hold fp32, but the
+// tensor cores' own sums do not: 160 sequences of up to 200 tokens, 6 heads, width 1488, random queries and cache ended
+// at 1.03 x 2^-16 of what was added up, where the fp32 FMAs of the other form end at 0.07 x 2^-16.
 //
 // The softmax reference of a row is a power of two that only moves when some weight would pass 2^15
 // (then the row's accumulator columns are rescaled in TMEM, exactly); the sums use the scores alone
@@ -84,10 +88,10 @@ constexpr float kTop = 15.f;               // a weight may reach 2^kTop
 // A new reference leaves the row's largest weight at 2^(kTop - kRoom): each bit of room saves moves of the
 // accumulators (a stall of the CTA) and raises the floor of the weights, 2^(kRoom - 32) of the largest, where
 // e5m2 ends.  As many bits as keep weights down to about 2^-15 of the largest within one unit of the output's
-// type: bf16 9, fp16 6; fp32 1.  bf16 with 6 / 9, random queries and cache of 64 x 4,608, width 1536: 24 heads
+// type: bf16 9, fp16 6.  bf16 with 6 / 9, random queries and cache of 64 x 4,608, width 1536: 24 heads
 // 168 / 158 us, 12 heads of ragged lengths 83.1 / 76.7.
 template <int QP>
-constexpr float kRoom = QP == 2 ? 9.f : QP == 3 ? 6.f : 1.f;
+constexpr float kRoom = QP == 2 ? 9.f : 6.f;
 constexpr float kNoRef = -3e38f;            // finite: a score of -inf weighs nothing against it
 constexpr float kSumRoom = 40.f;           // the sums' reference may lag by this many bits
 
@@ -361,9 +365,7 @@ __global__ void __launch_bounds__(kPrepThreads) attn_tc_prep_kernel(const __grid
   for (int j = 0; j < 8; ++j) x.v[j] = from_f<T>(0.f);
   if (o < p.a.cache.width >> 3) {
     if (p.q_vec) {
-#pragma unroll
-      for (int j = 0; j < (int)sizeof(T) / 2; ++j)
-        reinterpret_cast<int4*>(x.v)[j] = __ldg(reinterpret_cast<const int4*>(q) + j);
+      *reinterpret_cast<int4*>(x.v) = __ldg(reinterpret_cast<const int4*>(q));
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) x.v[j] = q[j];
@@ -858,7 +860,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             sum[r + e] += ex2(es[r + e]);
             v[e] = ex2(ev[r + e]);
           }
-          // fp16 holds three parts; those before come off in fp32
+          // an fp16 holds three parts; the one before them comes off in fp32
           __half2 h;
           if constexpr (S::WP == 3) h = __floats2half2_rn(v[0], v[1]);
 #pragma unroll
@@ -1180,7 +1182,7 @@ bool make_plan(const MlaCacheAttnArgs& a, Plan* pl) {
 }
 
 bool plan_for(int dtype, const MlaCacheAttnArgs& a, Plan* pl) {
-  return dtype == 0 ? make_plan<5>(a, pl) : dtype == 1 ? make_plan<2>(a, pl) : make_plan<3>(a, pl);
+  return dtype == 1 ? make_plan<2>(a, pl) : make_plan<3>(a, pl);
 }
 
 // wide: [B][L / 128][Tmax][128] as a view of the cache, boxes of `group` chunks x 64 tokens.  Else [B][Tmax][L]
@@ -1282,9 +1284,9 @@ cudaError_t launch_rh(const TcParams& p, const Plan& pl, cudaStream_t s) {
 
 }  // namespace
 
-// Code rows that TMA can address: 16-byte base and strides.
+// 16-bit queries, and code rows that TMA can address: 16-byte base and strides.
 bool mla_attn_tc_supported(int dtype, const MlaCacheAttnArgs& a) {
-  if (dtype < 0 || dtype > 2) return false;
+  if (dtype != 1 && dtype != 2) return false;
   if (a.cache.width % 16 || a.cache.width < 64 || a.cache.width > 8 * kPrepThreads) return false;
   if (a.cache.slots > (1 << 30)) return false;
   if ((reinterpret_cast<uintptr_t>(a.cache.codes) & 15) || (a.batch > 1 && a.cache.code_b % 16)) return false;
@@ -1341,8 +1343,7 @@ cudaError_t mla_attn_tc(int dtype, const MlaCacheAttnArgs& a, cudaStream_t s) {
   p.fetch = kFetch;
   p.direct = pl.direct ? 1 : 0;
   p.tmem = pl.tmem;
-  const int vec = dtype == 0 ? 4 : 8;
-  p.q_vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.q_b % vec == 0 && a.q_i % vec == 0 && a.q_h % vec == 0;
+  p.q_vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.q_b % 8 == 0 && a.q_i % 8 == 0 && a.q_h % 8 == 0;
   const bool one = a.batch == 1 || a.cache.code_b == 0;  // every sequence reads the same rows
   p.z_mul = one ? 0 : 1;
   p.t_first = one || p.a.cache.code_t <= a.cache.code_b ? 1 : 0;
@@ -1362,11 +1363,7 @@ cudaError_t mla_attn_tc(int dtype, const MlaCacheAttnArgs& a, cudaStream_t s) {
   p.prefix = reinterpret_cast<int*>(a.part_acc + wk.prefix);
   p.status = status_ptr();
   if (!p.status) return cudaErrorInvalidValue;
-  switch (dtype) {
-    case 0: return launch_rh<float, 5>(p, pl, s);
-    case 1: return launch_rh<__nv_bfloat16, 2>(p, pl, s);
-    default: return launch_rh<__half, 3>(p, pl, s);
-  }
+  return dtype == 1 ? launch_rh<__nv_bfloat16, 2>(p, pl, s) : launch_rh<__half, 3>(p, pl, s);
 }
 
 int* mla_cache_default_status() { return status_ptr(); }

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_mla_cache_gpu import E4M3, check_attention, make_cache, queries
+from test_mla_cache_gpu import E4M3, UNIT, check_attention, make_cache, quantise64, queries
 
 pytestmark = pytest.mark.gpu
 
