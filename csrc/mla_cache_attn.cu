@@ -33,15 +33,24 @@ int generic_splits(const MlaCacheAttnArgs& a) {
 size_t generic_smem(int width) {
   const size_t wp = (width + 3) / 4 * 4;
   return kRows * wp * sizeof(float) + kChunk * (wp + 4) + kChunk * kRows * sizeof(float) + kChunk * sizeof(float) +
-         3 * kRows * sizeof(float);
+         4 * kRows * sizeof(float);
+}
+
+// Compensated addition (Kahan): `lost` carries what rounding took off the sum so far.
+KIMI_D void add_kept(float& sum, float& lost, float x) {
+  const float y = x - lost, t = sum + y;
+  lost = (t - sum) - y;
+  sum = t;
 }
 
 // fp32 arithmetic on any width and alignment: the form for fp32 queries and for what TMA cannot address (widths, strides
 // or a base that are no multiples of 16 bytes; widths under 64).  A warp scores 4 tokens x 8 rows
 // per pass over the latent axis (a lane holds four adjacent columns: 128 FMAs per 12 shared-memory
-// loads); in the context phase a thread owns four adjacent columns of up to CP groups of 1,024.  The FMA
+// loads); in the context phase a thread owns four adjacent columns of up to CP groups of 1,024.  A chunk's products
+// are added up on their own and its total with the rounding kept: equal weights along a cache round the same way at
+// every step, so 131,072 plain additions end up to 3e-3 off, these within a few roundings of a chunk.  The FMA
 // pipes bound it: 16 x 2,048 tokens, 12 heads take 302 us at width 1,544, where TMA cannot address the rows,
-// and 32 us on the tensor cores at width 1,552.  fp32 queries: 4 x up to 1,000 tokens, 10 heads, width 640 35.9 us.
+// and 32 us on the tensor cores at width 1,552.  fp32 queries: 4 x up to 1,000 tokens, 10 heads, width 640 33.6 us.
 template <typename T, int CP>
 __global__ void __launch_bounds__(kThreads) attn_any_kernel(const __grid_constant__ MlaCacheAttnArgs a) {
   extern __shared__ __align__(16) unsigned char any_smem[];
@@ -50,7 +59,7 @@ __global__ void __launch_bounds__(kThreads) attn_any_kernel(const __grid_constan
   uint8_t* sx = reinterpret_cast<uint8_t*>(sq + kRows * wp);            // [kChunk][pitch]
   float* sp = reinterpret_cast<float*>(sx + kChunk * pitch);            // [kChunk][kRows]
   float* ssc = sp + kChunk * kRows;                                     // [kChunk] token scales
-  float* sstat = ssc + kChunk;                                          // max, sum, rescale [kRows] each
+  float* sstat = ssc + kChunk;  // max, sum, rescale, what the sum's last addition lost: [kRows] each
   const int split = blockIdx.x, tile = blockIdx.y, b = blockIdx.z, splits = gridDim.x;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rows = a.queries * a.heads, row0 = tile * kRows, nrow = min(kRows, rows - row0);
@@ -74,15 +83,15 @@ __global__ void __launch_bounds__(kThreads) attn_any_kernel(const __grid_constan
   for (int i = tid; i < kChunk * pitch; i += kThreads) sx[i] = 0;
   if (tid < kRows) {
     sstat[tid] = -INFINITY;
-    sstat[kRows + tid] = 0.f;
+    sstat[kRows + tid] = sstat[3 * kRows + tid] = 0.f;
   }
-  float acc[CP][4][kRows];
+  float acc[CP][4][kRows], low[CP][4][kRows];  // context, and what its last addition lost
 #pragma unroll
   for (int c = 0; c < CP; ++c)
 #pragma unroll
     for (int e = 0; e < 4; ++e)
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) acc[c][e][r] = 0.f;
+      for (int r = 0; r < kRows; ++r) acc[c][e][r] = low[c][e][r] = 0.f;
   const uint8_t* xb = a.cache.codes + b * a.cache.code_b;
   const float* cb = a.cache.scales + b * a.cache.scale_b;
   const bool words = width % 4 == 0 && a.cache.code_t % 4 == 0 && (reinterpret_cast<uintptr_t>(xb) & 3) == 0;
@@ -149,42 +158,57 @@ __global__ void __launch_bounds__(kThreads) attn_any_kernel(const __grid_constan
       if (lane == 0) {
         const float f = exp2f(m0 - base);
         sstat[warp] = m;
-        sstat[kRows + warp] = sstat[kRows + warp] * f + sum;
+        float total = sstat[kRows + warp] * f, lost = sstat[3 * kRows + warp] * f;
+        add_kept(total, lost, sum);
+        sstat[kRows + warp] = total;
         sstat[2 * kRows + warp] = f;
+        sstat[3 * kRows + warp] = lost;
       }
     } else if (warp < kRows) {
       sp[lane * kRows + warp] = 0.f;
-      if (lane == 0) sstat[2 * kRows + warp] = 0.f;
+      if (lane == 0) sstat[2 * kRows + warp] = 1.f;
     }
     __syncthreads();
     float f[kRows];
+    bool moved = false;
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) f[r] = sstat[2 * kRows + r];
+    for (int r = 0; r < kRows; ++r) {
+      f[r] = sstat[2 * kRows + r];
+      moved |= f[r] != 1.f;
+    }
 #pragma unroll
-    for (int c = 0; c < CP; ++c)
+    for (int c = 0; c < CP; ++c) {
+      const int l = 4 * tid + c * 4 * kThreads;
+      if (l >= wp) continue;
+      float part[4][kRows];  // of this chunk
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int r = 0; r < kRows; ++r) acc[c][e][r] *= f[r];
-    for (int t = 0; t < nt; ++t) {
-      const float4 w0 = *reinterpret_cast<const float4*>(sp + t * kRows);
-      const float4 w1 = *reinterpret_cast<const float4*>(sp + t * kRows + 4);
-      const float w[kRows] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+        for (int r = 0; r < kRows; ++r) part[e][r] = 0.f;
+      for (int t = 0; t < nt; ++t) {
+        const float4 w0 = *reinterpret_cast<const float4*>(sp + t * kRows);
+        const float4 w1 = *reinterpret_cast<const float4*>(sp + t * kRows + 4);
+        const float w[kRows] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+        const uint32_t u = *reinterpret_cast<const uint32_t*>(sx + t * pitch + l);
+        const float2 p = codes2(u), q = codes2(u >> 16);
 #pragma unroll
-      for (int c = 0; c < CP; ++c) {
-        const int l = 4 * tid + c * 4 * kThreads;
-        if (l < wp) {
-          const uint32_t u = *reinterpret_cast<const uint32_t*>(sx + t * pitch + l);
-          const float2 p = codes2(u), q = codes2(u >> 16);
-#pragma unroll
-          for (int r = 0; r < kRows; ++r) {
-            acc[c][0][r] += w[r] * p.x;
-            acc[c][1][r] += w[r] * p.y;
-            acc[c][2][r] += w[r] * q.x;
-            acc[c][3][r] += w[r] * q.y;
-          }
+        for (int r = 0; r < kRows; ++r) {
+          part[0][r] += w[r] * p.x;
+          part[1][r] += w[r] * p.y;
+          part[2][r] += w[r] * q.x;
+          part[3][r] += w[r] * q.y;
         }
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+          if (moved) {
+            acc[c][e][r] *= f[r];
+            low[c][e][r] *= f[r];
+          }
+          add_kept(acc[c][e][r], low[c][e][r], part[e][r]);
+        }
     }
   }
   __syncthreads();

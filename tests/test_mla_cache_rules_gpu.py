@@ -21,3 +21,42 @@ def test_last_columns_end_inside_a_warp(cuda, width, dtype):
     q = queries(b, 1, h, width, dtype, cuda)
     lens = torch.tensor([(i * 71) % (slots + 1) for i in range(b)], device=cuda)
     check_attention(ops.mla_cache_attention(q, codes, scales, lens, scale=0.6), q, codes, scales, lens, 0.6)
+
+
+def dominated(cuda, dtype, slots, first, floor=0.0, stretch=0):
+    """One token outweighs each of the others by 2^18 .. 2^33 (a head each); in half of the columns its code is zero, so
+    the output there is the tail alone, equal weights all of them.  160 query tokens of one sequence give every CTA whole
+    walks along the cache.  Returns each head's worst error as a share of the tolerance.
+
+    Tolerance per element: that of check_attention, plus what weights that are held to within `floor` of the largest one
+    may lose: at most `stretch` tokens share a stretch with the dominating one, each with a code of the column's size."""
+    from kimi_k3_b200 import ops
+    width, h, tq, scale, c = 64, 32, 160, 0.5, 4.0
+    g = torch.Generator(device=cuda).manual_seed(9)
+    x = torch.randn(1, slots, width, generator=g, device=cuda).abs() + 0.5
+    x[..., 0] = -c
+    at = 3 if first else slots // 2 + 3
+    x[0, at, 0] = c
+    x[0, at, 1:width // 2] = 0.0
+    codes, scales = (t.float() for t in quantise64(x))
+    codes = codes.to(E4M3)
+    q = torch.zeros(1, 1, h, width, device=cuda)
+    q[0, 0, :, 0] = torch.linspace(18.0, 33.0, h, device=cuda) * (math.log(2.0) / (2 * c * scale))
+    q = q.to(dtype)
+    lens = torch.tensor([slots], device=cuda)
+    out = ops.mla_cache_attention(q.expand(1, tq, h, width), codes, scales, lens, query_start=lens, scale=scale)
+    values = codes[0].double() * scales[0, :, None].double()
+    p = torch.softmax(q[0, 0].double() @ values.T * scale, -1)  # [h, slots]
+    ref, size = p @ values, p @ values.abs()
+    u = UNIT[dtype]
+    lost = floor * p.amax(-1, keepdim=True) * min(slots, stretch) * values.abs().amax(0)
+    tol = 0.5 * u * ref.abs() + u * size + lost
+    return ((out[0].double() - ref).abs() / tol).amax(dim=(0, 2)).tolist()
+
+
+@pytest.mark.parametrize("slots", [4608, 32768, 131072])
+@pytest.mark.parametrize("first", [True, False])
+def test_one_dominating_token_and_a_flat_tail_fp32(cuda, first, slots):
+    """Many equal weights round the same way at every addition: the sums along a cache keep their rounding."""
+    worst = dominated(cuda, torch.float32, slots, first)
+    assert max(worst) <= 1.0, worst
