@@ -32,8 +32,9 @@
 // with a reference of their own, so token scales far apart cost neither range nor accuracy.
 //
 // Work split: the tiles of all (sequence, row tile) pairs form one list, cut into equal contiguous
-// ranges, one per CTA, from the lengths on the device: ragged batches stay balanced and a launch (or
-// a captured graph) needs no lengths on the host.  A CTA that has a whole pair writes its output; the
+// ranges, one per CTA (more where they would be longer than a stretch, see kStretch), from the lengths on the device:
+// ragged batches stay balanced and a launch (or
+// a captured graph) needs no lengths on the host.  A range that has a whole pair writes its output; the
 // others leave a normalised context and its log-sum, joined by a second kernel in a fixed order.
 //
 // Three launches, each started while the one before still runs (programmatic dependent launch): the
@@ -85,13 +86,18 @@ constexpr int kJoinThreads = SL == 1 ? 128 : 256;
 constexpr int kPrepThreads = 256;          // 8 elements of a query row each: widths up to 2,048
 constexpr int kMisaligned = 9;             // status: shared memory off a 1,024-byte boundary
 constexpr float kTop = 15.f;               // a weight may reach 2^kTop
-// A new reference leaves the row's largest weight at 2^(kTop - kRoom): each bit of room saves moves of the
-// accumulators (a stall of the CTA) and raises the floor of the weights, 2^(kRoom - 32) of the largest, where
-// e5m2 ends.  As many bits as keep weights down to about 2^-15 of the largest within one unit of the output's
-// type: bf16 9, fp16 6.  bf16 with 6 / 9, random queries and cache of 64 x 4,608, width 1536: 24 heads
-// 168 / 158 us, 12 heads of ragged lengths 83.1 / 76.7.
+// A new reference leaves the row's largest weight at 2^(kTop - kRoom), or down to half of that: each bit of room saves
+// moves of the accumulators (a stall of the CTA) and raises the floor of the weights.  e5m2 ends in steps of 2^-16, so
+// a weight is held to within 2^(kRoom - 31) of the largest, and what many small weights add up to may be lost from the
+// context while the sum in the denominator has it.  kStretch bounds how many: each stretch of the cache this long
+// starts with references of its own.  A stretch then loses 2^(kRoom - 31) * kStretch of its weights' sum at most:
+// 2^-12 for bf16 with six bits, 2^-14 for fp16 with four, a sixteenth and an eighth of one unit of the type.
+// bf16 with six bits / nine: 64 x 4,608, width 1536, 24 heads 168 / 156 us, 12 heads of ragged lengths 85.5 / 78.3;
+// 8 x up to 2,048, 4 tokens of 12 heads, width 768 25.2 / 22.6.  fp16 with four / six: one sequence of 131,072, 16 heads,
+// width 1024 57.7 / 55.7.
 template <int QP>
-constexpr float kRoom = QP == 2 ? 9.f : 6.f;
+constexpr float kRoom = QP == 2 ? 6.f : 4.f;
+constexpr int kStretch = 8192 / kTile;     // tiles
 constexpr float kNoRef = -3e38f;            // finite: a score of -inf weighs nothing against it
 constexpr float kSumRoom = 40.f;           // the sums' reference may lag by this many bits
 
@@ -113,6 +119,7 @@ struct Plan {
   size_t smem = 0;
   bool direct = false;  // one CTA per pair, nothing to join
   int grid = 0;
+  int64_t ranges = 0;   // of the tile list, at most (see Walk)
 };
 
 struct TcParams {
@@ -127,9 +134,9 @@ struct TcParams {
   int64_t z_mul;       // 0 when every sequence reads the same cache rows
   uint8_t* q_parts;    // [pairs][q_bytes]: the shared-memory image of a pair's query parts
   float* coef;         // [pairs][R] score factors
-  float* part_o;       // [grid + pairs][rows_tile][L]
-  float* part_lse;     // [grid + pairs][rows_tile]
-  int* prefix;         // [pairs + 2]: first place of each pair, total, places per CTA
+  float* part_o;       // [ranges + pairs][rows_tile][L]
+  float* part_lse;     // [ranges + pairs][rows_tile]
+  int* prefix;         // [pairs + 2]: first place of each pair, total, places of a range
   int* status;
 };
 
@@ -312,28 +319,38 @@ KIMI_D int pair_tiles(const TcParams& p, int v, int64_t* len_out, int64_t* start
   return (int)((lim + kTile - 1) / kTile);
 }
 
-// The list of all pairs' tiles is cut into equal ranges, one per CTA.  Starting a pair costs a CTA about as
+// The list of all pairs' tiles is cut into equal ranges, one per CTA, or several one behind the other where one would
+// be longer than a stretch.  Starting a pair costs a CTA about as
 // much as kStart tiles (an epilogue, an empty pipeline), so each pair with tiles has kStart places in front;
 // none where every tile can have its own CTA.  0 / 2 / 4, 64 x 4,608, width 1536: 24 heads 147 / 143 / 142 us,
 // 12 heads 112 / 109 / 112, 3 heads 85.4 / 83.8 / 85.4.
 constexpr int kStart = 2;
 
-// This CTA's share of the list, walked pair by pair (every role walks it on its own).
+// This CTA's share of the list, walked segment by segment (every role walks it on its own).
+struct Share {
+  int v, t;        // the first pair and tile
+  int place, end;  // their place in the list, and where the CTA's ranges end
+  int per;         // places of a range
+};
 struct Walk {
-  int v, skip, left;  // pair, tiles of it that belong to CTAs before, places from there to the range's end
-  int t0, t1, tiles;  // the segment: tiles [t0, t1) of the pair's `tiles`
+  int v, place;  // pair, place in the list behind the segment
+  int t0, t1;    // the segment: tiles [t0, t1) of the pair
+  int range;     // that the segment lies in; -1 when it is the whole pair
   int64_t len, start;
-  KIMI_D bool next(const TcParams& p, int pairs) {
-    while (left > 0 && v < pairs) {
-      tiles = pair_tiles(p, v, &len, &start);
-      if (skip < tiles) {
-        t0 = skip;
-        t1 = min(tiles, skip + left);
-        left -= t1 - t0 + p.start;  // the next pair's places in front
-        skip = 0;
+  KIMI_D explicit Walk(const Share& s) : v(s.v), place(s.place), t0(0), t1(s.t), range(0), len(0), start(0) {}
+  KIMI_D bool next(const TcParams& p, const Share& s, int pairs) {
+    while (place < s.end && v < pairs) {
+      const int tiles = pair_tiles(p, v, &len, &start);
+      if (t1 < tiles) {
+        t0 = t1;
+        range = place / s.per;
+        t1 = min(tiles, t0 + min(s.end, (range + 1) * s.per) - place);
+        place += t1 - t0 + (t1 == tiles ? p.start : 0);  // the next pair's places in front
+        if (t1 - t0 == tiles) range = -1;
         return true;
       }
-      ++v;  // no tiles
+      ++v;  // no tiles (left)
+      t1 = 0;
     }
     return false;
   }
@@ -431,8 +448,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
   uint64_t* q_full = pv_done + 2;
   uint64_t* drain = q_full + 1;
   uint32_t* tslot = reinterpret_cast<uint32_t*>(drain + 1);
-  int* swalk = reinterpret_cast<int*>(tslot + 1);             // [3] first pair, skip, places
-  int* swsum = swalk + 3;                                     // [10] tiles counted by each warp
+  Share& share = *reinterpret_cast<Share*>(tslot + 1);
+  int* swsum = reinterpret_cast<int*>(&share + 1);            // [10] tiles counted by each warp
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int pairs = p.a.batch * p.row_tiles;
@@ -464,9 +481,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
   if (p.direct) {
     int64_t len, start;
     if (tid == 0) {
-      swalk[0] = blockIdx.x;
-      swalk[1] = 0;
-      swalk[2] = pair_tiles(p, blockIdx.x, &len, &start);  // all of it
+      const int n = pair_tiles(p, blockIdx.x, &len, &start);
+      share = {(int)blockIdx.x, 0, 0, n, max(n, 1)};  // all of it
     }
   } else {
     // Every thread counts the tiles of a run of pairs; a block scan places the runs in the tile list.
@@ -485,10 +501,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       if (lane >= o) incl += y;
     }
     if (lane == 31) swsum[warp] = incl;
-    if (tid == 0) {
-      swalk[0] = pairs;
-      swalk[1] = swalk[2] = 0;
-    }
+    if (tid == 0) share = {pairs, 0, 0, 0, 1};
     __syncthreads();
     int at = incl - own, total = 0;
 #pragma unroll
@@ -496,15 +509,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       if (i < warp) at += swsum[i];
       total += swsum[i];
     }
-    const int per = (total + p.grid - 1) / p.grid, mine = (int)blockIdx.x * per;  // < 2^31: the host bounds the tiles
+    // as many ranges for each CTA as keep them within a stretch; < 2^31: the host bounds the tiles
+    const int whole = (total + p.grid - 1) / p.grid, ranges = max(1, (whole + kStretch - 1) / kStretch);
+    const int per = (whole + ranges - 1) / ranges, mine = (int)blockIdx.x * ranges * per, end = mine + ranges * per;
     if (blockIdx.x == 0 || (mine >= at && mine < at + own)) {
       for (int v = v0; v < v1; ++v) {
         const int n = run == 1 ? last : pair_tiles(p, v, &len, &start), places = n > 0 ? n + p.start : 0;
         if (blockIdx.x == 0) p.prefix[v] = at;
         if (mine >= at && mine < at + places) {
-          swalk[0] = v;
-          swalk[1] = max(0, mine - at - p.start);
-          swalk[2] = mine + per - max(mine, at + p.start);
+          const int place = max(mine, at + p.start);
+          share = {v, place - at - p.start, place, end, per};
         }
         at += places;
       }
@@ -519,10 +533,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
   tc::tc_fence_after();
   const uint32_t tmem = *tslot;
   const uint32_t tm_s = tmem + (uint32_t)(p.boxes * p.np);  // score buffers behind the accumulators
-  Walk w;
-  w.v = swalk[0];
-  w.skip = swalk[1];
-  w.left = swalk[2];
+  Walk w(share);
 
   if (warp == 0) {
     // ---- loads
@@ -531,7 +542,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       uint32_t n = 0;  // stages loaded so far
       int st = 0;
       uint32_t ph = 1;  // parity of the last release of stage `st` before this use
-      while (ok && w.next(p, pairs)) {
+      while (ok && w.next(p, share, pairs)) {
         const int zb = (int)((w.v / p.row_tiles) * p.z_mul);
         for (int t = w.t0; ok && t < w.t1; ++t) {
           const bool fetch = p.fetch > 0 && t + p.fetch < w.t1;
@@ -557,7 +568,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             }
           }
         }
-        ++w.v;
       }
       // copies in flight land before the CTA ends
       for (uint32_t i = n > (uint32_t)p.stages ? n - p.stages : 0; i < n; ++i)
@@ -583,7 +593,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                      p_hi = (uint32_t)(bd_p >> 32);
       const uint32_t stage16 = (uint32_t)(p.group * (kBox >> 4));
       Walk ws = w, wo = w;
-      bool s_have = ws.next(p, pairs), o_have = wo.next(p, pairs);
+      bool s_have = ws.next(p, share, pairs), o_have = wo.next(p, share, pairs);
       int s_t = ws.t0, o_t = wo.t0;
       uint64_t since = 0;
       while (o_have) {
@@ -610,8 +620,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
           tc::mma_commit(&pv_done[pb]);
           ++o_n;
           if (++o_t == wo.t1) {
-            ++wo.v;
-            o_have = wo.next(p, pairs);
+            o_have = wo.next(p, share, pairs);
             o_t = wo.t0;
           }
           polls = 0;
@@ -640,8 +649,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
               s_open = false;
               ++s_n;
               if (++s_t == ws.t1) {
-                ++ws.v;
-                s_have = ws.next(p, pairs);
+                s_have = ws.next(p, share, pairs);
                 s_t = ws.t0;
                 ++s_seg;
               }
@@ -700,7 +708,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       bulk_load(sq, p.q_parts + (int64_t)v * p.q_bytes, p.q_bytes, q_full);
     };
     pdl_wait();  // the query parts are there
-    bool have = w.next(p, pairs);
+    bool have = w.next(p, share, pairs);
     if (have && warp == 2) {
       if (elect_one()) load_q(w.v);
       ++n_q;
@@ -710,8 +718,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       const int b = w.v / p.row_tiles, row0 = (w.v - b * p.row_tiles) * p.rows_tile;
       const int nrow = min(p.rows_tile, p.rows - row0);
       Walk nx = w;
-      ++nx.v;
-      const bool more = nx.next(p, pairs);
+      const bool more = nx.next(p, share, pairs);
       float coef[HR], ref[HR], reft[HR], sum[HR];
 #pragma unroll
       for (int r = 0; r < HR; ++r) {
@@ -893,8 +900,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         if ((lane & 15) == 0) sred[quad * R + rr + r] = x;
       }
       group_sync(bar_id);
-      const bool whole = w.t0 == 0 && w.t1 == w.tiles;
-      const int64_t part = (int64_t)blockIdx.x + w.v;
+      const bool whole = w.range < 0;
+      const int64_t part = (int64_t)w.range + w.v;
       if (quad == 0 && lane < RH) {
         const int r = r0 + lane;
         const float x = sred[r] + sred[R + r] + sred[2 * R + r] + sred[3 * R + r];
@@ -942,7 +949,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       w = nx;
       have = more;
     }
-    if (p.direct && swalk[2] == 0) {  // a pair without a key
+    if (p.direct && share.end == 0) {  // a pair without a key
       const int b = blockIdx.x / p.row_tiles, row0 = (blockIdx.x - b * p.row_tiles) * p.rows_tile;
       const int64_t n = (int64_t)min(p.rows_tile, p.rows - row0) * width;
       T* out = static_cast<T*>(p.a.out) + ((int64_t)b * p.rows + row0) * width;
@@ -963,7 +970,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
   }
 }
 
-// Joins the CTAs of a pair: weights 2^(lse_c - max), in the order of the CTAs.  A pair inside one CTA is
+// Joins the ranges of a pair: weights 2^(lse_c - max), in the order of the ranges.  A pair inside one range is
 // already written.  A block takes one row and COLS * V * 4 columns; with many parts (a few long sequences) SL
 // groups of threads take every SL-th part each and are added up in shared memory.
 template <typename T, int SL>
@@ -989,10 +996,10 @@ __global__ void __launch_bounds__(kJoinThreads<SL>) attn_tc_join_kernel(const __
 #pragma unroll
   for (int k = 0; k < V; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
   if constexpr (SL > 1) {  // all log-sums at once
-    const int parts = c1 - c0 + 1;  // <= kMaxGrid
-    for (int i = threadIdx.x; i < parts; i += kJoinThreads<SL>) {
-      slse[i] = lse[(int64_t)(c0 + i) * p.rows_tile];
-      m = fmaxf(m, slse[i]);
+    for (int i = threadIdx.x; i <= c1 - c0; i += kJoinThreads<SL>) {
+      const float x = lse[(int64_t)(c0 + i) * p.rows_tile];
+      if (i < kMaxGrid) slse[i] = x;
+      m = fmaxf(m, x);
     }
     m = warp_max(m);
     if ((threadIdx.x & 31) == 0) sstat[threadIdx.x >> 5] = m;
@@ -1009,7 +1016,7 @@ __global__ void __launch_bounds__(kJoinThreads<SL>) attn_tc_join_kernel(const __
     for (int i = 0; i < U; ++i) {
       const int ci = c + i * SL;
       const bool on = ci <= c1;
-      f[i] = !on ? -INFINITY : SL > 1 ? slse[ci - c0] : lse[(int64_t)ci * p.rows_tile];
+      f[i] = !on ? -INFINITY : SL > 1 && ci - c0 < kMaxGrid ? slse[ci - c0] : lse[(int64_t)ci * p.rows_tile];
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         const int l = l0 + k * COLS * 4;
@@ -1176,8 +1183,11 @@ bool make_plan(const MlaCacheAttnArgs& a, Plan* pl) {
   const int64_t pairs = (int64_t)a.batch * pl->row_tiles, tiles = (a.cache.slots + kTile - 1) / kTile;
   if (pairs > (1 << 20) || pairs * tiles > (1 << 29)) return false;
   const int sms = device_sms() < kMaxGrid ? device_sms() : kMaxGrid;
-  pl->direct = one_cta_per_pair(pairs, tiles, sms, pl->rows_tile, a.cache.width);
+  pl->direct = tiles <= kStretch && one_cta_per_pair(pairs, tiles, sms, pl->rows_tile, a.cache.width);
   pl->grid = pl->direct ? (int)pairs : (int)(pairs * tiles < sms ? pairs * tiles : sms);
+  // as the kernel divides the list, for sequences that fill their slots: shorter ones make no more
+  const int64_t whole = (pairs * (tiles + kStart) + pl->grid - 1) / pl->grid;
+  pl->ranges = pl->grid * ((whole + kStretch - 1) / kStretch);
   return true;
 }
 
@@ -1262,7 +1272,7 @@ cudaError_t launch(const TcParams& p, const Plan& pl, cudaStream_t s) {
   // 131,072, 16 heads, width 1024: all of it 47.3 us with SL = 16, 49.1 with 8; 700 tokens, 10 heads, width 640: 12.7
   // with 8, 13.6 with 2); many rows wide blocks (8 x 2304, 48 rows, width 768: 21.6 with 2, 26.9 with 8).
   const bool narrow = rows * ((width + 63) / 64) <= 600;
-  const int sl = pl.grid >= 32 * pairs ? (narrow ? 16 : 8) : pl.grid >= 6 * pairs ? (narrow ? 8 : 2) : 1;
+  const int sl = pl.ranges >= 32 * pairs ? (narrow ? 16 : 8) : pl.ranges >= 6 * pairs ? (narrow ? 8 : 2) : 1;
   switch (sl) {
     case 16: return launch_dependent(attn_tc_join_kernel<T, 16>, dim3(rows, (width + 63) / 64), 256, 0, s, p);
     case 8: return launch_dependent(attn_tc_join_kernel<T, 8>, dim3(rows, (width + 127) / 128), 256, 0, s, p);
@@ -1301,7 +1311,7 @@ struct Work {
   int64_t coef, part_o, part_lse, prefix, total;
 };
 static Work work_of(const MlaCacheAttnArgs& a, const Plan& pl) {
-  const int64_t pairs = (int64_t)a.batch * pl.row_tiles, units = pl.direct ? 0 : (pl.grid + pairs) * pl.rows_tile;
+  const int64_t pairs = (int64_t)a.batch * pl.row_tiles, units = pl.direct ? 0 : (pl.ranges + pairs) * pl.rows_tile;
   Work w;
   w.coef = pairs * pl.boxes * pl.ns * 32;
   w.part_o = w.coef + pairs * 2 * pl.rh;

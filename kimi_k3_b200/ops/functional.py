@@ -519,7 +519,13 @@ def mla_cache_attention(query_latent, codes, scales, lengths, *, query_start=Non
     The cached latent is key and value of every head.  Query token i of sequence b stands at position
     ``query_start[b] + i`` (default ``lengths[b] - Tq + i``: the last Tq cached tokens) and sees the slots
     below ``lengths[b]`` up to its own position; a query that sees none gets zeros.  Scores are
-    multiplied by ``scale``.  Softmax statistics and contexts are held in fp32."""
+    multiplied by ``scale``.  Softmax statistics and contexts are held in fp32.
+
+    fp32 queries run on fp32 FMAs.  bf16 and fp16 queries run on the tensor cores in 8-bit parts: a query
+    element keeps its type's bits down to 2^-18 (bf16) or 2^-27 (fp16) of its row's largest, a key's weight
+    (times the token's scale) 11 or 14 bits and no less than 2^-25 or 2^-27 of the largest weight of its
+    stretch of the cache, 8,192 tokens at most.  So a long tail of keys that far below one dominating key
+    may lose up to 2^-12 or 2^-14 of the stretch's weight."""
     _serving_only(query_latent, "mla_cache_attention")
     return _C().mla_cache_attention(query_latent, codes, scales, lengths, query_start, float(scale))
 

@@ -60,3 +60,13 @@ def test_one_dominating_token_and_a_flat_tail_fp32(cuda, first, slots):
     """Many equal weights round the same way at every addition: the sums along a cache keep their rounding."""
     worst = dominated(cuda, torch.float32, slots, first)
     assert max(worst) <= 1.0, worst
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("slots", [4608, 32768, 131072])
+@pytest.mark.parametrize("first", [True, False])
+def test_one_dominating_token_and_a_flat_tail(cuda, first, slots, dtype):
+    """A key's weight is held to within 2^-25 (bf16) or 2^-27 (fp16) of the largest weight of its stretch of the cache,
+    8,192 tokens at most."""
+    worst = dominated(cuda, dtype, slots, first, 2.0 ** (-25 if dtype == torch.bfloat16 else -27), 8192)
+    assert max(worst) <= 1.0, worst
