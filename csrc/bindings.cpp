@@ -1341,6 +1341,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("mla_cache_write", &mla_cache_write);
   m.def("mla_cache_read", &mla_cache_read);
   m.def("mla_cache_attention", &mla_cache_attention);
+  m.def("mla_cache_attention_form", [](at::ScalarType dtype, int64_t width) {
+    const int dt = dtype == at::kFloat ? 0 : dtype == at::kBFloat16 ? 1 : dtype == at::kHalf ? 2 : -1;
+    return dt < 0 || width <= 0 || width > (1 << 20) ? 0 : kimi::mla_cache_attn_form(dt, (int)width);
+  });
   m.def("mla_cache_status", [](bool clear) {
     const int v = kimi::mla_cache_status(clear);
     TORCH_CHECK(v >= 0, "reading the MLA cache status word failed");

@@ -193,6 +193,8 @@ struct MlaCacheAttnArgs {
 cudaError_t mla_cache_write(int dtype, const MlaCacheWriteArgs& a, cudaStream_t s);
 cudaError_t mla_cache_read(int dtype, const MlaCacheReadArgs& a, cudaStream_t s);
 bool mla_cache_attn_supported(int width);
+// How queries of this type and width are attended over a contiguous cache: 0 not at all, 1 fp32 FMAs, 2 tensor cores.
+int mla_cache_attn_form(int dtype, int width);
 int64_t mla_cache_attn_workspace(int dtype, const MlaCacheAttnArgs& a);
 cudaError_t mla_cache_attn(int dtype, const MlaCacheAttnArgs& a, cudaStream_t s);
 // Device status word of the attention's bounded waits (0 = ok), read and cleared by the host.

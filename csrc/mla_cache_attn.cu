@@ -292,6 +292,17 @@ cudaError_t launch_any(const MlaCacheAttnArgs& a, cudaStream_t s) {
 // 8 rows of fp32 query and a 32-token chunk have to fit shared memory.
 bool mla_cache_attn_supported(int width) { return width > 0 && width <= 2048; }
 
+int mla_cache_attn_form(int dtype, int width) {
+  if (!mla_cache_attn_supported(width)) return 0;
+  MlaCacheAttnArgs a;  // one row over a contiguous cache
+  a.cache.width = width;
+  a.cache.code_t = width;
+  a.cache.slots = 64;
+  a.cache.code_b = a.cache.slots * width;
+  a.batch = a.queries = a.heads = 1;
+  return mla_attn_tc_supported(dtype, a) ? 2 : 1;
+}
+
 int64_t mla_cache_attn_workspace(int dtype, const MlaCacheAttnArgs& a) {
   if (mla_attn_tc_supported(dtype, a)) return mla_attn_tc_workspace(dtype, a);
   const int splits = generic_splits(a);

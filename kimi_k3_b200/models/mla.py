@@ -529,6 +529,21 @@ def absorbed_latent_decode(query, latent_cache, cache_mask, key_up_weight, value
 # 603 / 2408, 1016 / 2624, 1672 / 2824, 2974 / 2793; 16 of 4,096, 24 heads, width 1536 901 / 3148, 2177 / 3310,
 # 3927 / 3436, 7472 / 3065.
 ABSORBED_QUERY_LIMIT = 64
+# The same where the attention runs on fp32 FMAs (fp32 layers, widths that are no multiples of 16), at 4, 8 and 16 query
+# tokens: fp32, 64 of 2,048, 10 heads, width 640 1903 / 4699, 3082 / 4710, 5418 / 4770; fp32, 16 of 4,096, 24 heads,
+# width 1536 3608 / 11372, 6856 / 11373, 11966 / 11418; bf16, 64 of 2,048, 10 heads, width 648 2059 / 2302,
+# 3309 / 2292, 5744 / 2416.
+ABSORBED_QUERY_LIMIT_FMA = 8
+
+
+def absorbed_query_limit(query: torch.Tensor, latent_dim: int) -> int:
+    """Query tokens per row up to which a quantized cache is attended in the latent space (0: never)."""
+    if not _ops.use_kernels(query):
+        return ABSORBED_QUERY_LIMIT
+    form = _ops.mla_cache_attention_form(query.dtype, latent_dim)
+    if form is None:
+        return 0
+    return ABSORBED_QUERY_LIMIT if form == "tensor_cores" else min(ABSORBED_QUERY_LIMIT, ABSORBED_QUERY_LIMIT_FMA)
 
 
 def absorbed_quantized_attention(query, cache: QuantizedMLACache, key_up_weight, value_up_weight, num_heads, *,
@@ -655,7 +670,7 @@ class GatedMLA(nn.Module):
             # the append advances the offsets in place
             start = prev.clone() if t > 1 else None
             updated = cache.append(latent, attention_mask)
-            if (t <= ABSORBED_QUERY_LIMIT and not need_probs and self.absorbed_decode and not c.projection_bias
+            if (t <= absorbed_query_limit(query, c.kv_latent_dim) and not need_probs and self.absorbed_decode and not c.projection_bias
                     and not output_diagnostics):
                 raw = absorbed_quantized_attention(query, updated, self.projections.latent_kv.key_up.weight,
                                                    self.projections.latent_kv.value_up.weight, c.num_heads,

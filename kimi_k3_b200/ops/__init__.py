@@ -17,7 +17,7 @@ from . import _loader
 from .functional import (attnres_mix, conv_silu_norm, conv_silu_norm_step, flash_attention, kda_chunk, kda_decay,
                          kda_decode_step, linear, linear_cross_entropy, linear_group, linear_group_supported,
                          linear_supported, mark_seen, mla_absorbed_decode, mla_cache_attention,
-                         mla_cache_check, mla_cache_read, mla_cache_write, mla_decode_supported,
+                         mla_cache_attention_form, mla_cache_check, mla_cache_read, mla_cache_write, mla_decode_supported,
                          moe_grouped_experts, qb_histogram, rms_norm, router_topk, sample_tokens, sigmoid_mul,
                          situ_glu)
 
@@ -39,5 +39,5 @@ __all__ = [
     "conv_silu_norm", "kda_decay", "flash_attention", "mla_absorbed_decode", "router_topk", "qb_histogram",
     "moe_grouped_experts", "attnres_mix", "linear_cross_entropy", "conv_silu_norm_step", "mla_decode_supported",
     "sample_tokens", "mark_seen", "mla_cache_write", "mla_cache_read", "mla_cache_attention",
-    "mla_cache_check",
+    "mla_cache_attention_form", "mla_cache_check",
 ]

@@ -512,6 +512,13 @@ def mla_cache_read(codes, scales, lengths=None, *, dtype=torch.bfloat16, tokens:
     return _C().mla_cache_read(codes, scales, lengths, dtype, codes.shape[1] if tokens is None else int(tokens))
 
 
+def mla_cache_attention_form(dtype: torch.dtype, latent_dim: int) -> str | None:
+    """How :func:`mla_cache_attention` takes queries of this type and width: ``"tensor_cores"`` (16-bit types, widths
+    from 64 that are multiples of 16), ``"fma"`` (fp32 and other widths up to 2,048; several times slower for many
+    query rows), or None: it refuses them."""
+    return (None, "fma", "tensor_cores")[_C().mla_cache_attention_form(dtype, int(latent_dim))]
+
+
 def mla_cache_attention(query_latent, codes, scales, lengths, *, query_start=None, scale: float = 1.0) -> torch.Tensor:
     """Attention of ``query_latent`` ``[B,Tq,H,L]`` (queries absorbed into the latent space, any strides
     outside the last axis) over an 8-bit MLA cache -> contexts ``[B,Tq,H,L]`` in the query's type.

@@ -70,3 +70,75 @@ def test_one_dominating_token_and_a_flat_tail(cuda, first, slots, dtype):
     8,192 tokens at most."""
     worst = dominated(cuda, dtype, slots, first, 2.0 ** (-25 if dtype == torch.bfloat16 else -27), 8192)
     assert max(worst) <= 1.0, worst
+
+
+# ------------------------------------------------------------------------------------------ the layer's choice
+def _layer(cuda, width, d_model=128, heads=2):
+    from kimi_k3_b200.models.mla import GatedMLA, GatedMLAConfig
+    torch.manual_seed(11)
+    return GatedMLA(GatedMLAConfig(d_model=d_model, num_heads=heads, q_head_dim=64, v_head_dim=64,
+                                   kv_latent_dim=width)).to(cuda).eval()
+
+
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_layer_with_a_latent_wider_than_the_attention_takes(cuda, tokens, monkeypatch):
+    """Widths that the attention kernel refuses are read back and rebuilt: the layer runs, and equals its PyTorch form
+    within a few fp32 roundings of the output's size."""
+    from kimi_k3_b200 import ops
+    from kimi_k3_b200.models.mla import QuantizedMLACache
+    layer = _layer(cuda, 2176, d_model=1152, heads=18)
+    assert ops.mla_cache_attention_form(torch.float32, 2176) is None
+    b, prompt = 2, 37
+    x0, x = torch.randn(b, prompt, 1152, device=cuda), torch.randn(b, tokens, 1152, device=cuda)
+    with torch.no_grad():
+        first = QuantizedMLACache.from_cache(layer(x0, use_cache=True).cache, 48)
+        outs = []
+        for kernels in ("1", "0"):
+            monkeypatch.setenv("KIMI_K3_KERNELS", kernels)
+            cache = first.clone()
+            outs.append(layer(x, cache=cache, use_cache=True).hidden_states)
+            assert cache.sequence_offset.tolist() == [prompt + tokens] * b
+    err = (outs[0] - outs[1]).abs().max().item() / outs[1].abs().max().item()
+    assert err <= 2.0 ** -11, err
+
+
+def test_decoder_with_a_latent_wider_than_the_attention_takes(cuda):
+    from kimi_k3_b200.config.model_yaml import build_model_config_from_mapping
+    from kimi_k3_b200.config.profiles import profile_model_mapping
+    from kimi_k3_b200.infer import GenerationConfig, GraphDecoder
+    from kimi_k3_b200.models import KimiK3
+    m = profile_model_mapping("t4_wikitext")
+    m["model"].update(d_model=1152, num_heads=18, num_hybrid_groups=1, vocab_size=1000)
+    m["model"]["moe"].update(latent_dim=64, shared_expert_hidden_dim=96, routed_expert_hidden_dim=128)
+    m["model"]["mla"]["kv_latent_dim"] = 2176
+    torch.manual_seed(5)
+    model = KimiK3(build_model_config_from_mapping(m)).to(cuda).eval()
+    ids = torch.randint(5, 1000, (2, 21), device=cuda)
+    for use_graph in (True, False):
+        out = GraphDecoder(model, max_length=40, generation_config=GenerationConfig(max_new_tokens=6), cache_dtype=E4M3,
+                           use_graph=use_graph).generate(ids)
+        assert out.generated_tokens == 6
+        states = [lc.state for lc in out.cache.layer_caches if lc.attention_type == "gated_mla"]
+        assert states and all(s.sequence_offset.tolist() == [26, 26] for s in states)
+
+
+@pytest.mark.parametrize("dtype,width,tokens,attends", [
+    (torch.bfloat16, 128, 64, True), (torch.bfloat16, 128, 65, False), (torch.bfloat16, 136, 8, True),
+    (torch.bfloat16, 136, 9, False), (torch.float32, 128, 8, True), (torch.float32, 128, 9, False)])
+def test_layer_attends_up_to_the_limit_of_the_form(cuda, dtype, width, tokens, attends, monkeypatch):
+    """64 query tokens where the tensor cores attend, 8 where fp32 FMAs do; both forms against fp32 PyTorch."""
+    from kimi_k3_b200.models import mla
+    layer = _layer(cuda, width)
+    calls = []
+    attend = mla.QuantizedMLACache.attend
+    monkeypatch.setattr(mla.QuantizedMLACache, "attend", lambda self, q, **kw: calls.append(q.dtype) or attend(self, q, **kw))
+    b, prompt = 2, 50
+    x0, x = torch.randn(b, prompt, 128, device=cuda), torch.randn(b, tokens, 128, device=cuda)
+    with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16, enabled=dtype == torch.bfloat16):
+        first = mla.QuantizedMLACache.from_cache(layer(x0, use_cache=True).cache, prompt + tokens)
+        out = layer(x, cache=first.clone(), use_cache=True).hidden_states.float()
+        assert calls == ([dtype] if attends else [])
+        monkeypatch.setenv("KIMI_K3_KERNELS", "0")
+        want = layer(x, cache=first.clone(), use_cache=True).hidden_states.float()
+    err = (out - want).abs().max().item() / want.abs().max().item()
+    assert err <= (2.0 ** -6 if dtype == torch.bfloat16 else 2.0 ** -11), err
