@@ -72,6 +72,18 @@ def test_one_dominating_token_and_a_flat_tail(cuda, first, slots, dtype):
     assert max(worst) <= 1.0, worst
 
 
+def test_more_parts_than_one_block_lists(cuda):
+    """A sequence so long that its stretches outnumber the log-sums a joining block keeps at hand."""
+    from kimi_k3_b200 import ops
+    slots, width, h = 4_300_000, 64, 2
+    g = torch.Generator(device=cuda).manual_seed(2)
+    codes = torch.randint(0, 0x70, (1, slots, width), generator=g, device=cuda, dtype=torch.uint8).view(E4M3)
+    scales = torch.full((1, slots), 2.0 ** -9, device=cuda)
+    q = queries(1, 1, h, width, torch.bfloat16, cuda, spread=6.0)
+    lens = torch.tensor([slots - 5], device=cuda)
+    check_attention(ops.mla_cache_attention(q, codes, scales, lens), q, codes, scales, lens, 1.0)
+
+
 # ------------------------------------------------------------------------------------------ the layer's choice
 def _layer(cuda, width, d_model=128, heads=2):
     from kimi_k3_b200.models.mla import GatedMLA, GatedMLAConfig
