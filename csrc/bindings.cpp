@@ -1345,10 +1345,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     const int dt = dtype == at::kFloat ? 0 : dtype == at::kBFloat16 ? 1 : dtype == at::kHalf ? 2 : -1;
     return dt < 0 || width <= 0 || width > (1 << 20) ? 0 : kimi::mla_cache_attn_form(dt, (int)width);
   });
-  m.def("mla_cache_status", [](bool clear) {
-    const int v = kimi::mla_cache_status(clear);
-    TORCH_CHECK(v >= 0, "reading the MLA cache status word failed");
-    return v;
+  // View of the current device's status word of the attention (int32 [1], not owned).
+  m.def("mla_cache_status_word", []() {
+    int* p = kimi::mla_cache_default_status();
+    TORCH_CHECK(p, "the MLA cache status word is unavailable on this device");
+    return at::from_blob(p, {1}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, c10::cuda::current_device()));
   });
   m.def("sample_tokens", &sample_tokens);
   m.def("seen_mark", &seen_mark);

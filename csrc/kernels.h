@@ -197,8 +197,7 @@ bool mla_cache_attn_supported(int width);
 int mla_cache_attn_form(int dtype, int width);
 int64_t mla_cache_attn_workspace(int dtype, const MlaCacheAttnArgs& a);
 cudaError_t mla_cache_attn(int dtype, const MlaCacheAttnArgs& a, cudaStream_t s);
-// Device status word of the attention's bounded waits (0 = ok), read and cleared by the host.
-int mla_cache_status(bool clear);
+// Address of the current device's status word of the attention's bounded waits (0 = ok), read and cleared by the host.
 int* mla_cache_default_status();
 
 // ---------------------------------------------------------------- expert-parallel comm (ep_comm.cu)

@@ -1378,14 +1378,4 @@ cudaError_t mla_attn_tc(int dtype, const MlaCacheAttnArgs& a, cudaStream_t s) {
 
 int* mla_cache_default_status() { return status_ptr(); }
 
-int mla_cache_status(bool clear) {
-  int v = 0;
-  if (cudaMemcpyFromSymbol(&v, g_mla_cache_status, sizeof(int)) != cudaSuccess) return -1;
-  if (clear && v) {
-    const int zero = 0;
-    if (cudaMemcpyToSymbol(g_mla_cache_status, &zero, sizeof(int)) != cudaSuccess) return -1;
-  }
-  return v;
-}
-
 }  // namespace kimi

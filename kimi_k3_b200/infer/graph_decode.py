@@ -291,7 +291,7 @@ class GraphDecoder:
             decode_s = time.perf_counter() - t1
             if self.cache_dtype is not None and dev.type == "cuda":
                 from .. import ops
-                ops.mla_cache_check()
+                ops.mla_cache_check(dev)
         finally:
             if was_training:
                 model.train()

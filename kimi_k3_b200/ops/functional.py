@@ -537,10 +537,17 @@ def mla_cache_attention(query_latent, codes, scales, lengths, *, query_start=Non
     return _C().mla_cache_attention(query_latent, codes, scales, lengths, query_start, float(scale))
 
 
-def mla_cache_check() -> None:
-    """Raise if a bounded wait of an attention kernel on the current device gave up since the last check
-    (its results are void).  Waits for the device: call it where the host synchronises anyway."""
-    status = _C().mla_cache_status(True)
+def mla_cache_check(device=None) -> None:
+    """Raise if a bounded wait of an attention kernel on ``device`` (default: the current one) gave up since
+    the last check (its results are void), and clear the record.  Waits for every stream of the device: call
+    it where the host synchronises anyway."""
+    with torch.cuda.device(device):
+        torch.cuda.synchronize()
+        word = _C().mla_cache_status_word()
+        status = int(word.item())
+        if status:
+            word.zero_()
+            torch.cuda.synchronize()
     if status:
         raise RuntimeError(f"mla_cache_attention: a bounded wait gave up (status {status}); its results are void")
 

@@ -154,3 +154,46 @@ def test_layer_attends_up_to_the_limit_of_the_form(cuda, dtype, width, tokens, a
         want = layer(x, cache=first.clone(), use_cache=True).hidden_states.float()
     err = (out - want).abs().max().item() / want.abs().max().item()
     assert err <= (2.0 ** -6 if dtype == torch.bfloat16 else 2.0 ** -11), err
+
+
+# ------------------------------------------------------------------------------------------ waits that gave up
+@pytest.fixture
+def status_word(cuda):
+    """The device's record of waits that gave up; left clear."""
+    from kimi_k3_b200.ops import _loader
+    word = _loader.require().mla_cache_status_word()
+    yield word
+    torch.cuda.synchronize()
+    word.zero_()
+    torch.cuda.synchronize()
+
+
+def test_check_waits_for_every_stream(cuda, status_word):
+    """A record made late on a stream of its own is seen, reported once and cleared."""
+    from kimi_k3_b200 import ops
+    ops.mla_cache_check()
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)
+        status_word.fill_(3)
+    with pytest.raises(RuntimeError, match="status 3"):
+        ops.mla_cache_check(torch.device("cuda", torch.cuda.current_device()))
+    ops.mla_cache_check()
+    assert status_word.item() == 0
+
+
+def test_decoder_checks_its_own_device(cuda, status_word, monkeypatch):
+    from kimi_k3_b200 import ops
+    from kimi_k3_b200.infer import GenerationConfig, GraphDecoder
+    from test_decode_gpu import _small_model
+    model = _small_model(cuda)
+    asked, check = [], ops.mla_cache_check
+    monkeypatch.setattr(ops, "mla_cache_check", lambda device=None: asked.append(device) or check(device))
+    ids = torch.randint(5, 1000, (2, 9), device=cuda)
+    cfg = GenerationConfig(max_new_tokens=3)
+    GraphDecoder(model, max_length=16, generation_config=cfg, cache_dtype=E4M3).generate(ids)
+    assert [torch.device(d) for d in asked] == [next(model.parameters()).device]
+    asked.clear()
+    GraphDecoder(model, max_length=16, generation_config=cfg).generate(ids)
+    assert not asked
