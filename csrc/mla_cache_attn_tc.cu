@@ -53,7 +53,8 @@
 //
 // Roles of an attention CTA (10 warps): warp 0 loads, warp 1 issues the MMAs, warps 2-9 are two groups
 // of four that share the rows: scores -> weights, rescaling and the epilogue.
-// Every mbarrier wait is bounded and reports through the status word.
+// Every mbarrier wait is bounded and reports through the status word.  What a CTA had in hand when one gave up is written as
+// NaN, and so is everything while the word stays set.
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -450,6 +451,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
   uint32_t* tslot = reinterpret_cast<uint32_t*>(drain + 1);
   Share& share = *reinterpret_cast<Share*>(tslot + 1);
   int* swsum = reinterpret_cast<int*>(&share + 1);            // [10] tiles counted by each warp
+  volatile int* svoid = swsum + kThreads / 32;                // a wait has given up: what this CTA has is void
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int pairs = p.a.batch * p.row_tiles;
@@ -467,6 +469,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     tc::mbar_init(&p_full[tid - 64], 8);
     tc::mbar_init(&pv_done[tid - 64], 1);
   }
+  // a record that nobody has cleared: every wait would give up, so nothing is started
+  if (tid == 128) *svoid = tc::status_peek(p.status);
   if (tid == 96) {
     tc::mbar_init(q_full, 1);
     tc::mbar_init(drain, 1);
@@ -534,10 +538,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
   const uint32_t tmem = *tslot;
   const uint32_t tm_s = tmem + (uint32_t)(p.boxes * p.np);  // score buffers behind the accumulators
   Walk w(share);
+  const bool idle = *svoid != 0;
 
   if (warp == 0) {
     // ---- loads
-    if (elect_one()) {
+    if (!idle && elect_one()) {
       bool ok = true;
       uint32_t n = 0;  // stages loaded so far
       int st = 0;
@@ -578,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     // ---- MMAs.  Issued under elect.sync with descriptors that are sums of precomputed words, an MMA costs
     // what the tensor core takes (28 clocks for a score step of 48 columns, 40 for a context step); behind
     // a plain lane test the issue alone took 90 to 170.
-    if (elect_one()) {
+    if (!idle && elect_one()) {
       // Two streams over the same tiles, scores and context, each taken as soon as its operands are there:
       // a context product goes first (it frees its tile's part of the ring), else the next stage of scores.
       int s_st = 0, o_st = 0, s_i = 0;  // ring stages of the streams; stage of the score tile
@@ -693,12 +698,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       row_at[r] = (uint32_t)((n >> 3) * 1024 + (n & 7) * 128 + ((quad ^ (n & 7)) << 4) + (lane & 15));
     }
     // A wait that fails only makes this warp skip its later waits: every warp walks all tiles, so the
-    // groups' named barriers always meet and the kernel ends (its results are void, as the status says).
+    // groups' named barriers always meet and the kernel ends (its results are NaN, and the status says so).
     bool ok = true;
     uint32_t n_tile = 0;
     int stage = 0;  // first stage of the tile
     auto wait = [&](uint64_t* bar, uint32_t use, int code) {  // the warp is converged again behind it, and agrees
       ok = __all_sync(0xffffffffu, ok && tc::mbar_wait(bar, use & 1, p.status, code));
+      if (!ok) *svoid = 1;  // before this warp arrives anywhere
       tc::tc_fence_after();
     };
     // One copy at a time: the next is issued behind a wait that shows the one before to be read.
@@ -708,7 +714,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       bulk_load(sq, p.q_parts + (int64_t)v * p.q_bytes, p.q_bytes, q_full);
     };
     pdl_wait();  // the query parts are there
-    bool have = w.next(p, share, pairs);
+    if (idle) {  // NaN for every row with a key
+      while (w.next(p, share, pairs)) {
+        const int b = w.v / p.row_tiles, row0 = (w.v - b * p.row_tiles) * p.rows_tile;
+        const int nrow = min(p.rows_tile, p.rows - row0);
+        if (w.range < 0) {
+          T* out = static_cast<T*>(p.a.out) + ((int64_t)b * p.rows + row0) * width;
+          for (int64_t i = tid - 64; i < (int64_t)nrow * width; i += 256) out[i] = from_f<T>(__uint_as_float(0x7FC00000u));
+        } else if (tid - 64 < nrow) {
+          p.part_lse[((int64_t)w.range + w.v) * p.rows_tile + tid - 64] = __uint_as_float(0x7FC00000u);
+        }
+      }
+      __syncwarp();
+    }
+    bool have = !idle && w.next(p, share, pairs);
     if (have && warp == 2) {
       if (elect_one()) load_q(w.v);
       ++n_q;
@@ -912,6 +931,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       }
       group_sync(bar_id);
       wait(&pv_done[(n_tile - 1) & 1], (n_tile - 1) >> 1, tc::kTimeoutTmemEmpty);
+      // a warp that gave up before this segment's last product was issued has said so
+      const bool sound = *svoid == 0;
+      if (!sound && !whole && quad == 0 && lane < RH && r0 + lane < nrow)
+        p.part_lse[part * p.rows_tile + r0 + lane] = __uint_as_float(0x7FC00000u);
+      __syncwarp();
       {
         const int elt = whole ? (int)sizeof(T) : 4, have_rows = nrow - r0, l0 = quad * 32 + lane;
         const int64_t row = whole ? (int64_t)b * p.rows + row0 + r0 : part * p.rows_tile + r0;
@@ -937,6 +961,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
               if (g < p.stack) x += v[g][r];
             // no key: the accumulator may hold a stale column, the row is zeros
             x = f.y == 0.f ? 0.f : x * f.x * f.y;
+            if (!sound) x = __uint_as_float(0x7FC00000u);
             if (r < rows) {
               if (whole) *reinterpret_cast<T*>(at) = from_f<T>(x);
               else *reinterpret_cast<float*>(at) = x;
@@ -1105,7 +1130,7 @@ bool fit(int boxes, Plan* pl) {
     int tile_stages = 0, group = 0, stages = 0, p_bufs = 2;
     size_t fixed = 0;
     for (; p_bufs >= 1; --p_bufs) {
-      fixed = (size_t)boxes * S::NS * 128 + p_bufs * p_bytes + (2 + 4 + 8) * S::R * 4 + (2 * kMaxStages + 10) * 8 + 64;
+      fixed = (size_t)boxes * S::NS * 128 + p_bufs * p_bytes + (2 + 4 + 8) * S::R * 4 + (2 * kMaxStages + 10) * 8 + 80;
       stages = 0;
       for (int g = kMaxGroup; g >= 1 && fixed < kSmemMax; --g) {
         tile_stages = (boxes + g - 1) / g;

@@ -532,15 +532,19 @@ def mla_cache_attention(query_latent, codes, scales, lengths, *, query_start=Non
     element keeps its type's bits down to 2^-18 (bf16) or 2^-27 (fp16) of its row's largest, a key's weight
     (times the token's scale) 11 or 14 bits and no less than 2^-25 or 2^-27 of the largest weight of its
     stretch of the cache, 8,192 tokens at most.  So a long tail of keys that far below one dominating key
-    may lose up to 2^-12 or 2^-14 of the stretch's weight."""
+    may lose up to 2^-12 or 2^-14 of the stretch's weight.
+
+    Waits inside the tensor-core kernel are bounded.  Should one run out, the rows it concerns are NaN, and so
+    are those of later calls until :func:`mla_cache_check` has reported it."""
     _serving_only(query_latent, "mla_cache_attention")
     return _C().mla_cache_attention(query_latent, codes, scales, lengths, query_start, float(scale))
 
 
 def mla_cache_check(device=None) -> None:
     """Raise if a bounded wait of an attention kernel on ``device`` (default: the current one) gave up since
-    the last check (its results are void), and clear the record.  Waits for every stream of the device: call
-    it where the host synchronises anyway."""
+    the last check, and clear the record.  Results from the give-up to the check are NaN.  Waits for every
+    stream of the device: call it where the host synchronises anyway (the serving decoder does, after each
+    generation)."""
     with torch.cuda.device(device):
         torch.cuda.synchronize()
         word = _C().mla_cache_status_word()

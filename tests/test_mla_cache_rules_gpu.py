@@ -197,3 +197,21 @@ def test_decoder_checks_its_own_device(cuda, status_word, monkeypatch):
     asked.clear()
     GraphDecoder(model, max_length=16, generation_config=cfg).generate(ids)
     assert not asked
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(40, 2, 10, 640, 190), (3, 1, 6, 640, 9000), (2, 40, 24, 128, 700)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_results_are_nan_until_a_give_up_is_reported(cuda, status_word, shape, dtype):
+    """With the record of a wait that gave up still set, rows with a key come back NaN, whole and joined ones alike; the
+    check reports it, and the next call is right."""
+    from kimi_k3_b200 import ops
+    b, tq, h, width, slots = shape
+    codes, scales = make_cache(b, slots, width, cuda)
+    q = queries(b, tq, h, width, dtype, cuda)
+    lens = torch.tensor([(slots, tq + 5, 65 + tq)[i % 3] for i in range(b)], device=cuda)
+    status_word.fill_(2)
+    assert torch.isnan(ops.mla_cache_attention(q, codes, scales, lens, scale=0.6)).all()
+    with pytest.raises(RuntimeError, match="status 2"):
+        ops.mla_cache_check()
+    check_attention(ops.mla_cache_attention(q, codes, scales, lens, scale=0.6), q, codes, scales, lens, 0.6)
