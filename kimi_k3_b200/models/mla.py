@@ -292,12 +292,12 @@ class QuantizedMLACache(StaticMLACache):
         if cache.latent_kv.shape[1] > self.latent_kv.shape[1]:
             raise ValueError(f"prompt of {cache.latent_kv.shape[1]} tokens exceeds the serving cache "
                              f"({self.latent_kv.shape[1]})")
-        self.sequence_offset.zero_()
-        self._write(cache.latent_kv, self.sequence_offset, cache.sequence_offset)
+        self._write(cache.latent_kv, torch.zeros_like(self.sequence_offset), cache.sequence_offset)
         self.sequence_offset.copy_(cache.sequence_offset)
         return self
 
     def _write(self, latent, offsets, counts=None) -> None:
+        _ops.serving_only(latent, "writing a quantized MLA cache")
         if _ops.use_kernels(latent):
             _ops.mla_cache_write(latent, self.latent_kv, self.scales, offsets, counts)
             return
@@ -336,6 +336,7 @@ class QuantizedMLACache(StaticMLACache):
         if _ops.use_kernels(query_latent):
             return _ops.mla_cache_attention(query_latent, self.latent_kv, self.scales, self.sequence_offset,
                                             query_start=query_start, scale=scale)
+        _ops.serving_only(query_latent, "attending over a quantized MLA cache")
         tq = query_latent.shape[1]
         wd = torch.promote_types(query_latent.dtype, torch.float32)
         start = self.sequence_offset - tq if query_start is None else query_start

@@ -18,8 +18,8 @@ from .functional import (attnres_mix, conv_silu_norm, conv_silu_norm_step, flash
                          kda_decode_step, linear, linear_cross_entropy, linear_group, linear_group_supported,
                          linear_supported, mark_seen, mla_absorbed_decode, mla_cache_attention,
                          mla_cache_attention_form, mla_cache_check, mla_cache_read, mla_cache_write, mla_decode_supported,
-                         moe_grouped_experts, qb_histogram, rms_norm, router_topk, sample_tokens, sigmoid_mul,
-                         situ_glu)
+                         moe_grouped_experts, qb_histogram, rms_norm, router_topk, sample_tokens, serving_only,
+                         sigmoid_mul, situ_glu)
 
 
 def kernels_enabled() -> bool:

@@ -486,7 +486,8 @@ def mla_absorbed_decode(query, latent_cache, cache_mask, key_up_weight, value_up
 
 
 # --------------------------------------------------------------------------- 8-bit MLA latent cache
-def _serving_only(x: torch.Tensor, name: str) -> None:
+def serving_only(x: torch.Tensor, name: str) -> None:
+    """Refuse a tensor whose gradient would be dropped: what the 8-bit latent cache holds has none."""
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} has no backward: the 8-bit latent cache is a serving structure "
                            "(call it under torch.no_grad() or torch.inference_mode())")
@@ -501,7 +502,7 @@ def mla_cache_write(latent, codes, scales, offsets, counts=None) -> None:
     buffer are dropped.  A token's scale is the least power of two 2^k, k >= -126, under which its
     largest magnitude fits e4m3 (448 * 2^k); a token holding a NaN or an infinity gets scale NaN and
     codes 0.  ``offsets`` and ``counts`` are int32 or int64 ``[B]`` device tensors."""
-    _serving_only(latent, "mla_cache_write")
+    serving_only(latent, "mla_cache_write")
     _C().mla_cache_write(latent, codes, scales, offsets, counts)
 
 
@@ -536,7 +537,7 @@ def mla_cache_attention(query_latent, codes, scales, lengths, *, query_start=Non
 
     Waits inside the tensor-core kernel are bounded.  Should one run out, the rows it concerns are NaN, and so
     are those of later calls until :func:`mla_cache_check` has reported it."""
-    _serving_only(query_latent, "mla_cache_attention")
+    serving_only(query_latent, "mla_cache_attention")
     return _C().mla_cache_attention(query_latent, codes, scales, lengths, query_start, float(scale))
 
 

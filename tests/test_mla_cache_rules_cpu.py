@@ -1,0 +1,33 @@
+"""The 8-bit MLA latent cache off the GPU: refusals and values away from the ordinary ones."""
+import math
+
+import pytest
+import torch
+
+from kimi_k3_b200.models.mla import GatedMLA, GatedMLAConfig, MLACache, QuantizedMLACache
+
+
+def _cache(b=2, tokens=5, slots=12, width=8, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    plain = MLACache.empty(b, width, dtype=torch.float32).append(torch.randn(b, tokens, width, generator=g))
+    return QuantizedMLACache.from_cache(plain, slots)
+
+
+def test_gradients_are_refused_not_dropped():
+    """The cache keeps no gradient: a latent or a query that needs one is refused and leaves the cache as it was."""
+    cache = _cache()
+    codes, offsets = cache.latent_kv.view(torch.uint8).clone(), cache.sequence_offset.clone()
+    x = torch.randn(2, 3, 8, requires_grad=True)
+    for call in (lambda: cache.append(x), lambda: cache.attend(x[:, :, None]),
+                 lambda: cache.load(MLACache.empty(2, 8, dtype=torch.float32).append(x))):
+        with pytest.raises(RuntimeError, match="no backward"):
+            call()
+    assert torch.equal(cache.latent_kv.view(torch.uint8), codes) and torch.equal(cache.sequence_offset, offsets)
+    layer = GatedMLA(GatedMLAConfig(d_model=16, num_heads=2, q_head_dim=8, v_head_dim=8, kv_latent_dim=8))
+    with pytest.raises(RuntimeError, match="no backward"):
+        layer(torch.randn(2, 1, 16), cache=cache, use_cache=True)
+    assert torch.equal(cache.sequence_offset, offsets)
+    with torch.no_grad():
+        cache.append(x)
+        cache.attend(x[:, :, None])
+    assert cache.sequence_offset.tolist() == [8, 8]
