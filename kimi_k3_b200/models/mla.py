@@ -349,6 +349,8 @@ class QuantizedMLACache(StaticMLACache):
         some = seen.any(dim=-1)[:, :, None, None]
         p = torch.softmax(torch.where(some, scores, torch.zeros_like(scores)), dim=-1)
         p = torch.where(seen[:, :, None, :], p, torch.zeros_like(p))
+        # a token of scale NaN reaches the rows that see it through p alone: 0 * NaN would reach the others too
+        values = torch.where(torch.isnan(values), torch.zeros_like(values), values)
         return torch.einsum("biht,btl->bihl", p, values).to(query_latent.dtype)
 
     def clone(self) -> "QuantizedMLACache":

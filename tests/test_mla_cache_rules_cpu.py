@@ -31,3 +31,13 @@ def test_gradients_are_refused_not_dropped():
         cache.append(x)
         cache.attend(x[:, :, None])
     assert cache.sequence_offset.tolist() == [8, 8]
+
+
+def test_a_nan_token_reaches_only_the_queries_that_see_it():
+    cache = _cache(tokens=6)
+    q = torch.randn(2, 3, 4, 8, generator=torch.Generator().manual_seed(1))
+    want = cache.attend(q)
+    cache.scales[0, 5] = math.nan  # seen by the last query token alone
+    cache.latent_kv.view(torch.uint8)[0, 5] = 0
+    got = cache.attend(q)
+    assert torch.isnan(got[0, 2]).all() and torch.equal(got[0, :2], want[0, :2]) and torch.equal(got[1], want[1])
