@@ -59,8 +59,11 @@ def run_distributed_generation(model_config_path, checkpoint_path, prompt, infer
                                cache_dtype: torch.dtype | None = None):
     """Initialise the mesh from ``inference_yaml.distributed``, load, shard, generate.
 
-    ``cache_dtype`` is the serving decoder's (``use_graph``).  Returns ``(output, context)``; the caller reports on ``context.is_global_zero`` and closes
-    the context."""
+    ``cache_dtype`` is the serving decoder's and needs ``use_graph`` (on the CPU the decoder then runs its steps
+    eagerly).  Returns ``(output, context)``; the caller reports on ``context.is_global_zero`` and closes the
+    context."""
+    if cache_dtype is not None and not use_graph:
+        raise ValueError("cache_dtype needs the serving decoder (use_graph=True)")
     from ..parallel.environment import setup_distributed
     from .config import ModelLoadConfig
     from .generation import inference_autoregressive
@@ -73,7 +76,7 @@ def run_distributed_generation(model_config_path, checkpoint_path, prompt, infer
                                   load_config=ModelLoadConfig(device=device, precision=precision))
     model = prepare_distributed_model(loaded.model, dist_cfg, context)
     gen = replace(gen, device=str(next(model.parameters()).device))
-    if use_graph and torch.device(gen.device).type == "cuda":
+    if use_graph and (torch.device(gen.device).type == "cuda" or cache_dtype is not None):
         from .graph_decode import GraphDecoder
         ids = encode_prompt(prompt, tokenizer=tokenizer, add_bos_token=gen.add_bos_token)
         ml = max_length or int(ids.shape[1]) + gen.max_new_tokens

@@ -41,3 +41,23 @@ def test_a_nan_token_reaches_only_the_queries_that_see_it():
     cache.latent_kv.view(torch.uint8)[0, 5] = 0
     got = cache.attend(q)
     assert torch.isnan(got[0, 2]).all() and torch.equal(got[0, :2], want[0, :2]) and torch.equal(got[1], want[1])
+
+
+def test_generation_honours_the_cache_dtype_or_refuses_it(tmp_path):
+    """Without the serving decoder there is no 8-bit cache to hold; with it there is one on the CPU too."""
+    from kimi_k3_b200.config.model_yaml import build_model_from_yaml
+    from kimi_k3_b200.config.profiles import write_pipeline
+    from kimi_k3_b200.infer import GenerationConfig, InferenceYamlConfig
+    from kimi_k3_b200.infer.distributed import run_distributed_generation
+    from kimi_k3_b200.parallel.config import DistributedConfig
+    write_pipeline("cpu_smoke", tmp_path)
+    model = build_model_from_yaml(tmp_path / "model.yaml")
+    torch.save({"model_state_dict": model.state_dict(), "format_version": 1}, tmp_path / "ckpt.pt")
+    iy = InferenceYamlConfig(GenerationConfig(max_new_tokens=4, device="cpu"), DistributedConfig(), None)
+    args = (tmp_path / "model.yaml", tmp_path / "ckpt.pt", [5, 17, 9, 33], iy)
+    with pytest.raises(ValueError, match="use_graph"):
+        run_distributed_generation(*args, cache_dtype=torch.float8_e4m3fn)
+    out, context = run_distributed_generation(*args, use_graph=True, cache_dtype=torch.float8_e4m3fn)
+    context.close()
+    states = [lc.state for lc in out.cache.layer_caches if lc.attention_type == "gated_mla"]
+    assert states and all(isinstance(s, QuantizedMLACache) for s in states)
