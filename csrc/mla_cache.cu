@@ -80,7 +80,7 @@ struct Oct<float> {
 // Slot of token j of sequence b, or -1.
 KIMI_D int64_t write_slot(const MlaCacheWriteArgs& a, int b, int64_t j) {
   if (a.counts.p && j >= get(a.counts, b)) return -1;
-  const int64_t s = get(a.offsets, b) + j;
+  const int64_t s = cut(get(a.offsets, b)) + j;
   return s >= 0 && s < a.cache.slots ? s : -1;
 }
 

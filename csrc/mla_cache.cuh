@@ -22,6 +22,17 @@ KIMI_D int64_t get(const MlaCacheInts& v, int b) {
   return v.is64 ? static_cast<const int64_t*>(v.p)[b] : (int64_t) static_cast<const int32_t*>(v.p)[b];
 }
 
+// Length of sequence b as given, and the position of its first query token.  Both are cut to +-2^40, far past any slot:
+// a position of INT64_MAX sees every key, and adding to it does not wrap.
+KIMI_D int64_t cut(int64_t v) {
+  constexpr int64_t far = (int64_t)1 << 40;
+  return v < -far ? -far : v > far ? far : v;
+}
+KIMI_D int64_t first_position(const MlaCacheAttnArgs& a, int b, int64_t* len) {
+  *len = cut(get(a.lengths, b));
+  return a.start.p ? cut(get(a.start, b)) : *len - a.queries;
+}
+
 // Two e4m3 codes (low half of `w`) to floats.
 KIMI_D float2 codes2(uint32_t w) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w & 0xFFFFu), __NV_E4M3);

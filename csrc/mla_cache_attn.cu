@@ -63,8 +63,8 @@ __global__ void __launch_bounds__(kThreads) attn_any_kernel(const __grid_constan
   const int split = blockIdx.x, tile = blockIdx.y, b = blockIdx.z, splits = gridDim.x;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rows = a.queries * a.heads, row0 = tile * kRows, nrow = min(kRows, rows - row0);
-  int64_t len = get(a.lengths, b);
-  const int64_t start = a.start.p ? get(a.start, b) : len - a.queries;
+  int64_t len;
+  const int64_t start = first_position(a, b, &len);
   len = len < 0 ? 0 : len > a.cache.slots ? a.cache.slots : len;
   // keys that the last row of the tile sees, and this split's share of them in whole chunks
   const int64_t seen = start + (row0 + nrow - 1) / a.heads + 1;

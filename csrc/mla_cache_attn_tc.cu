@@ -309,8 +309,8 @@ KIMI_D uint32_t take_e5m2x2(__half2& h) {
 // Tiles of pair v: the keys its last row sees.
 KIMI_D int pair_tiles(const TcParams& p, int v, int64_t* len_out, int64_t* start_out) {
   const int b = v / p.row_tiles, rt = v - b * p.row_tiles;
-  int64_t len = get(p.a.lengths, b);
-  const int64_t start = p.a.start.p ? get(p.a.start, b) : len - p.a.queries;
+  int64_t len;
+  const int64_t start = first_position(p.a, b, &len);
   len = len < 0 ? 0 : len > p.a.cache.slots ? p.a.cache.slots : len;
   const int last = min(p.rows, (rt + 1) * p.rows_tile) - 1;
   const int64_t seen = start + last / p.a.heads + 1;

@@ -340,6 +340,7 @@ class QuantizedMLACache(StaticMLACache):
         tq = query_latent.shape[1]
         wd = torch.promote_types(query_latent.dtype, torch.float32)
         start = self.sequence_offset - tq if query_start is None else query_start
+        start = start.long().clamp(-2 ** 40, 2 ** 40)  # as far as matters: a position past every slot does not wrap
         last = start[:, None] + torch.arange(tq, device=start.device)
         key = torch.arange(self.latent_kv.shape[1], device=start.device)
         seen = self.valid_mask()[:, None, :] & (key <= last[..., None])  # [B,Tq,T]

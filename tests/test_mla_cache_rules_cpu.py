@@ -61,3 +61,15 @@ def test_generation_honours_the_cache_dtype_or_refuses_it(tmp_path):
     context.close()
     states = [lc.state for lc in out.cache.layer_caches if lc.attention_type == "gated_mla"]
     assert states and all(isinstance(s, QuantizedMLACache) for s in states)
+
+
+def test_positions_past_every_slot_do_not_wrap():
+    cache = _cache()
+    q = torch.randn(2, 3, 4, 8, generator=torch.Generator().manual_seed(2))
+    ends = torch.iinfo(torch.int64)
+    all_keys = cache.attend(q, query_start=torch.tensor([100, 5]))
+    got = cache.attend(q, query_start=torch.tensor([ends.max, ends.max]))
+    assert torch.equal(got, all_keys) and got.any()
+    assert not cache.attend(q, query_start=torch.tensor([ends.min, -3])).any()
+    ints = cache.attend(q, query_start=torch.full((2,), torch.iinfo(torch.int32).max, dtype=torch.int32))
+    assert torch.equal(ints, all_keys)

@@ -84,6 +84,25 @@ def test_more_parts_than_one_block_lists(cuda):
     check_attention(ops.mla_cache_attention(q, codes, scales, lens), q, codes, scales, lens, 1.0)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_positions_past_every_slot_do_not_wrap(cuda, dtype):
+    from kimi_k3_b200 import ops
+    b, tq, h, width, slots = 3, 3, 4, 768, 100
+    codes, scales = make_cache(b, slots, width, cuda)
+    q = queries(b, tq, h, width, dtype, cuda)
+    ends = torch.iinfo(torch.int64)
+    lens = torch.tensor([100, 40, ends.max], device=cuda)  # a length past the slots is the slots
+    far = torch.tensor([ends.max, ends.max - 1, 100], device=cuda)
+    want = ops.mla_cache_attention(q, codes, scales, lens, query_start=torch.full_like(lens, slots))
+    assert torch.equal(ops.mla_cache_attention(q, codes, scales, lens, query_start=far), want) and want.any()
+    assert torch.equal(ops.mla_cache_attention(q, codes, scales, lens, query_start=far.clamp(max=2 ** 31 - 1).int()), want)
+    assert not ops.mla_cache_attention(q, codes, scales, lens, query_start=torch.full_like(lens, ends.min)).any()
+    before = codes.view(torch.uint8).clone()
+    x = torch.randn(b, 2, width, device=cuda).to(dtype)
+    ops.mla_cache_write(x, codes, scales, torch.tensor([ends.max, ends.min, slots], device=cuda))
+    assert torch.equal(codes.view(torch.uint8), before)
+
+
 # ------------------------------------------------------------------------------------------ the layer's choice
 def _layer(cuda, width, d_model=128, heads=2):
     from kimi_k3_b200.models.mla import GatedMLA, GatedMLAConfig
