@@ -120,6 +120,7 @@ struct Plan {
   size_t smem = 0;
   bool direct = false;  // one CTA per pair, nothing to join
   int grid = 0;
+  int stretch = 0;      // places of a range at most
   int64_t ranges = 0;   // of the tile list, at most (see Walk)
 };
 
@@ -131,6 +132,7 @@ struct TcParams {
   int fetch;           // tiles ahead that are brought into L2
   int r_pad, stack, runs, ns, np, p_bytes, p_bufs, q_bytes, grid;
   int start;           // places of a pair in front of its tiles (see kStart)
+  int stretch;         // places of a range at most (see kStretch)
   uint32_t tmem;
   int64_t z_mul;       // 0 when every sequence reads the same cache rows
   uint8_t* q_parts;    // [pairs][q_bytes]: the shared-memory image of a pair's query parts
@@ -513,8 +515,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       if (i < warp) at += swsum[i];
       total += swsum[i];
     }
-    // as many ranges for each CTA as keep them within a stretch; < 2^31: the host bounds the tiles
-    const int whole = (total + p.grid - 1) / p.grid, ranges = max(1, (whole + kStretch - 1) / kStretch);
+    // as many ranges for each CTA as keep its segments within a stretch; < 2^31: the host bounds the tiles
+    const int whole = total / p.grid + (total % p.grid != 0), ranges = max(1, (whole - 1) / p.stretch + 1);
     const int per = (whole + ranges - 1) / ranges, mine = (int)blockIdx.x * ranges * per, end = mine + ranges * per;
     if (blockIdx.x == 0 || (mine >= at && mine < at + own)) {
       for (int v = v0; v < v1; ++v) {
@@ -1212,7 +1214,8 @@ bool make_plan(const MlaCacheAttnArgs& a, Plan* pl) {
   pl->grid = pl->direct ? (int)pairs : (int)(pairs * tiles < sms ? pairs * tiles : sms);
   // as the kernel divides the list, for sequences that fill their slots: shorter ones make no more
   const int64_t whole = (pairs * (tiles + kStart) + pl->grid - 1) / pl->grid;
-  pl->ranges = pl->grid * ((whole + kStretch - 1) / kStretch);
+  pl->stretch = tiles <= kStretch ? 1 << 30 : kStretch;  // no pair is longer than a stretch: only the CTAs divide them
+  pl->ranges = pl->grid * ((whole + pl->stretch - 1) / pl->stretch);
   return true;
 }
 
@@ -1375,6 +1378,7 @@ cudaError_t mla_attn_tc(int dtype, const MlaCacheAttnArgs& a, cudaStream_t s) {
   p.q_bytes = pl.boxes * pl.ns * 128;
   p.grid = pl.grid;
   p.start = (a.cache.slots + kTile - 1) / kTile * a.batch * pl.row_tiles <= pl.grid ? 0 : kStart;
+  p.stretch = pl.stretch;
   p.fetch = kFetch;
   p.direct = pl.direct ? 1 : 0;
   p.tmem = pl.tmem;
