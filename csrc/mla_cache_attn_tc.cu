@@ -131,14 +131,15 @@ struct TcParams {
   int wide;            // one copy per stage (L a multiple of 128), else one per box
   int fetch;           // tiles ahead that are brought into L2
   int r_pad, stack, runs, ns, np, p_bytes, p_bufs, q_bytes, grid;
+  int ranges;          // of the tile list, at most
   int start;           // places of a pair in front of its tiles (see kStart)
   int stretch;         // places of a range at most (see kStretch)
   uint32_t tmem;
   int64_t z_mul;       // 0 when every sequence reads the same cache rows
   uint8_t* q_parts;    // [pairs][q_bytes]: the shared-memory image of a pair's query parts
   float* coef;         // [pairs][R] score factors
-  float* part_o;       // [ranges + pairs][rows_tile][L]
-  float* part_lse;     // [ranges + pairs][rows_tile]
+  float* part_o;       // [ranges + min(ranges, pairs)][rows_tile][L] (see part_of)
+  float* part_lse;     // [ranges + min(ranges, pairs)][rows_tile]
   int* prefix;         // [pairs + 2]: first place of each pair, total, places of a range
   int* status;
 };
@@ -358,6 +359,13 @@ struct Walk {
     return false;
   }
 };
+
+// Number of the part that a range holds of a pair that it does not hold whole.  A range holds one such part that does not
+// start the pair, its first, and one that does, its last: the former are numbered by the range, the latter behind them by the
+// range or the pair, whichever are fewer.
+KIMI_D int64_t part_of(const TcParams& p, int range, int v, bool starts, int pairs) {
+  return !starts ? range : (int64_t)p.ranges + (pairs < p.ranges ? v : range);
+}
 
 template <typename T>
 struct alignas(16) Oct8 {
@@ -724,7 +732,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
           T* out = static_cast<T*>(p.a.out) + ((int64_t)b * p.rows + row0) * width;
           for (int64_t i = tid - 64; i < (int64_t)nrow * width; i += 256) out[i] = from_f<T>(__uint_as_float(0x7FC00000u));
         } else if (tid - 64 < nrow) {
-          p.part_lse[((int64_t)w.range + w.v) * p.rows_tile + tid - 64] = __uint_as_float(0x7FC00000u);
+          p.part_lse[part_of(p, w.range, w.v, w.t0 == 0, pairs) * p.rows_tile + tid - 64] = __uint_as_float(0x7FC00000u);
         }
       }
       __syncwarp();
@@ -922,7 +930,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       }
       group_sync(bar_id);
       const bool whole = w.range < 0;
-      const int64_t part = (int64_t)w.range + w.v;
+      const int64_t part = part_of(p, w.range, w.v, w.t0 == 0, pairs);
       if (quad == 0 && lane < RH) {
         const int r = r0 + lane;
         const float x = sred[r] + sred[R + r] + sred[2 * R + r] + sred[3 * R + r];
@@ -1010,21 +1018,20 @@ __global__ void __launch_bounds__(kJoinThreads<SL>) attn_tc_join_kernel(const __
   const int b = v / p.row_tiles, row0 = (v - b * p.row_tiles) * p.rows_tile, width = p.a.cache.width;
   const int pairs = p.a.batch * p.row_tiles;
   const int col = threadIdx.x % COLS, grp = threadIdx.x / COLS, l0 = (blockIdx.y * COLS * V + col) * 4;
-  const float* lse = p.part_lse + (int64_t)v * p.rows_tile + r;
-  const float* po = p.part_o + ((int64_t)v * p.rows_tile + r) * width;
   pdl_wait();
   if (row0 + r >= p.rows) return;
   const int at = p.prefix[v], places = p.prefix[v + 1] - at, per = p.prefix[pairs + 1];
   const int n = places - p.start;  // tiles, if any
   const int c0 = n > 0 ? (at + p.start) / per : 0, c1 = n > 0 ? (at + places - 1) / per : -1;
   if (n > 0 && c0 == c1) return;
+  auto row_of = [&](int c) { return part_of(p, c, v, c == c0, pairs) * p.rows_tile + r; };
   float4 acc[V];
   float m = -INFINITY, sum = 0.f;
 #pragma unroll
   for (int k = 0; k < V; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
   if constexpr (SL > 1) {  // all log-sums at once
     for (int i = threadIdx.x; i <= c1 - c0; i += kJoinThreads<SL>) {
-      const float x = lse[(int64_t)(c0 + i) * p.rows_tile];
+      const float x = p.part_lse[row_of(c0 + i)];
       if (i < kMaxGrid) slse[i] = x;
       m = fmaxf(m, x);
     }
@@ -1043,11 +1050,12 @@ __global__ void __launch_bounds__(kJoinThreads<SL>) attn_tc_join_kernel(const __
     for (int i = 0; i < U; ++i) {
       const int ci = c + i * SL;
       const bool on = ci <= c1;
-      f[i] = !on ? -INFINITY : SL > 1 && ci - c0 < kMaxGrid ? slse[ci - c0] : lse[(int64_t)ci * p.rows_tile];
+      f[i] = !on ? -INFINITY : SL > 1 && ci - c0 < kMaxGrid ? slse[ci - c0] : p.part_lse[row_of(ci)];
+      const float* po = p.part_o + row_of(ci) * width;
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         const int l = l0 + k * COLS * 4;
-        x[i][k] = on && l < width ? *reinterpret_cast<const float4*>(po + (int64_t)ci * p.rows_tile * width + l)
+        x[i][k] = on && l < width ? *reinterpret_cast<const float4*>(po + l)
                                   : make_float4(0.f, 0.f, 0.f, 0.f);
       }
     }
@@ -1339,7 +1347,8 @@ struct Work {
   int64_t coef, part_o, part_lse, prefix, total;
 };
 static Work work_of(const MlaCacheAttnArgs& a, const Plan& pl) {
-  const int64_t pairs = (int64_t)a.batch * pl.row_tiles, units = pl.direct ? 0 : (pl.ranges + pairs) * pl.rows_tile;
+  const int64_t pairs = (int64_t)a.batch * pl.row_tiles, 
+                units = pl.direct ? 0 : (pl.ranges + std::min(pl.ranges, pairs)) * pl.rows_tile;
   Work w;
   w.coef = pairs * pl.boxes * pl.ns * 32;
   w.part_o = w.coef + pairs * 2 * pl.rh;
@@ -1378,6 +1387,7 @@ cudaError_t mla_attn_tc(int dtype, const MlaCacheAttnArgs& a, cudaStream_t s) {
   p.q_bytes = pl.boxes * pl.ns * 128;
   p.grid = pl.grid;
   p.start = (a.cache.slots + kTile - 1) / kTile * a.batch * pl.row_tiles <= pl.grid ? 0 : kStart;
+  p.ranges = (int)pl.ranges;
   p.stretch = pl.stretch;
   p.fetch = kFetch;
   p.direct = pl.direct ? 1 : 0;

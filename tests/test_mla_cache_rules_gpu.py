@@ -103,6 +103,28 @@ def test_positions_past_every_slot_do_not_wrap(cuda, dtype):
     assert torch.equal(codes.view(torch.uint8), before)
 
 
+def test_workspace_does_not_grow_with_the_row_tiles(cuda):
+    """Parts of contexts are held for what the CTAs cut, two a CTA at most, however many row tiles a prompt piece makes.
+    Beside the output a call holds its query parts, as many bytes as the queries rounded up to the tile's rows."""
+    from kimi_k3_b200 import ops
+    b, tq, h, width, slots = 24, 60, 24, 640, 4000
+    codes, scales = make_cache(b, 8, width, cuda)
+    codes = codes.view(torch.uint8).repeat(1, slots // 8, 1).view(E4M3)
+    scales = scales.repeat(1, slots // 8)
+    q = queries(b, tq, h, width, torch.bfloat16, cuda)
+    lens = torch.full((b,), slots, device=cuda)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out = ops.mla_cache_attention(q, codes, scales, lens, scale=0.6)
+    used = torch.cuda.max_memory_allocated() - before
+    sms = torch.cuda.get_device_properties(cuda).multi_processor_count
+    size = q.numel() * q.element_size()
+    assert used <= 2 * size * 33 // 32 + 2 * sms * 32 * (width + 1) * 4 + (8 << 20), used
+    rows = slice(0, 2)
+    check_attention(out[rows], q[rows], codes[rows], scales[rows], lens[rows], 0.6)
+
+
 # ------------------------------------------------------------------------------------------ the layer's choice
 def _layer(cuda, width, d_model=128, heads=2):
     from kimi_k3_b200.models.mla import GatedMLA, GatedMLAConfig
