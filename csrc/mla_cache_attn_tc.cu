@@ -1179,7 +1179,8 @@ bool fit(int boxes, Plan* pl) {
 // a launch.  In ns, as measured: 1.2 a tile and latent, 2,000 the join, 1 / 3,000 a byte of the parts, there and back.
 // One CTA a pair / split, bf16: 64 x 256 tokens, 16 heads, L 1024 15.0 / 20.4 us; 100 x 400, 10, 640 18.1 / 24.9;
 // 32 x 128, 12, 768 10.1 / 11.9; 200 x 500, 10, 640 35.2 / 35.9; 16 x 528, 10, 640 18.7 / 16.2; 4 x 300, 24, 1536
-// 31.7 / 24.6; 1 x 512, 10, 640 16.5 / 12.7.  From the slots: the lengths are on the device.
+// 31.7 / 24.6; 1 x 512, 10, 640 16.5 / 12.7.  From the slots: the lengths are on the device.  So a buffer longer than what it
+// holds is split: 64 x 300 tokens, 24 heads, L 1536 44.0 us in 300 slots, 52 - 54 in 1,024 .. 65,536.
 bool one_cta_per_pair(int64_t pairs, int64_t tiles, int sms, int rows, int width) {
   const int64_t whole = (pairs + sms - 1) / sms * (tiles + kStart);
   const int64_t split = std::max<int64_t>((pairs * (tiles + kStart) + sms - 1) / sms, 1 + kStart);
@@ -1308,7 +1309,10 @@ cudaError_t launch(const TcParams& p, const Plan& pl, cudaStream_t s) {
   // 131,072, 16 heads, width 1024: all of it 47.3 us with SL = 16, 49.1 with 8; 700 tokens, 10 heads, width 640: 12.7
   // with 8, 13.6 with 2); many rows wide blocks (8 x 2304, 48 rows, width 768: 21.6 with 2, 26.9 with 8).
   const bool narrow = rows * ((width + 63) / 64) <= 600;
-  const int sl = pl.ranges >= 32 * pairs ? (narrow ? 16 : 8) : pl.ranges >= 6 * pairs ? (narrow ? 8 : 2) : 1;
+  // From the CTAs, not the ranges: a serving buffer is mostly longer than what it holds, and a sequence that fills many
+  // stretches takes far longer than its join.  64 sequences of 300 tokens in 65,536 slots, 24 heads, width 1536: 53.2 / 66.6 us
+  // by CTAs / by ranges.
+  const int sl = pl.grid >= 32 * pairs ? (narrow ? 16 : 8) : pl.grid >= 6 * pairs ? (narrow ? 8 : 2) : 1;
   switch (sl) {
     case 16: return launch_dependent(attn_tc_join_kernel<T, 16>, dim3(rows, (width + 63) / 64), 256, 0, s, p);
     case 8: return launch_dependent(attn_tc_join_kernel<T, 8>, dim3(rows, (width + 127) / 128), 256, 0, s, p);
