@@ -131,14 +131,14 @@ struct TcParams {
   int wide;            // one copy per stage (L a multiple of 128), else one per box
   int fetch;           // tiles ahead that are brought into L2
   int r_pad, stack, runs, ns, np, p_bytes, p_bufs, q_bytes, grid;
-  int ranges;          // of the tile list, at most
+  int part_c;          // numbers of parts that a range takes up (see part_of)
   int start;           // places of a pair in front of its tiles (see kStart)
   int stretch;         // places of a range at most (see kStretch)
   uint32_t tmem;
   int64_t z_mul;       // 0 when every sequence reads the same cache rows
   uint8_t* q_parts;    // [pairs][q_bytes]: the shared-memory image of a pair's query parts
   float* coef;         // [pairs][R] score factors
-  float* part_o;       // [ranges + min(ranges, pairs)][rows_tile][L] (see part_of)
+  float* part_o;       // [ranges + min(ranges, pairs)][rows_tile][L]
   float* part_lse;     // [ranges + min(ranges, pairs)][rows_tile]
   int* prefix;         // [pairs + 2]: first place of each pair, total, places of a range
   int* status;
@@ -360,11 +360,10 @@ struct Walk {
   }
 };
 
-// Number of the part that a range holds of a pair that it does not hold whole.  A range holds one such part that does not
-// start the pair, its first, and one that does, its last: the former are numbered by the range, the latter behind them by the
-// range or the pair, whichever are fewer.
-KIMI_D int64_t part_of(const TcParams& p, int range, int v, bool starts, int pairs) {
-  return !starts ? range : (int64_t)p.ranges + (pairs < p.ranges ? v : range);
+// Number of the part that range c holds of a pair v that it does not hold whole.  A range holds one such part that does not
+// start the pair, its first, and one that does, its last: two numbers a range, or, where the pairs are fewer, c + v.
+KIMI_D int64_t part_of(const TcParams& p, int c, int v, bool starts) {
+  return p.part_c == 1 ? (int64_t)c + v : 2 * (int64_t)c + (starts ? 1 : 0);
 }
 
 template <typename T>
@@ -524,8 +523,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       total += swsum[i];
     }
     // as many ranges for each CTA as keep its segments within a stretch; < 2^31: the host bounds the tiles
-    const int whole = total / p.grid + (total % p.grid != 0), ranges = max(1, (whole - 1) / p.stretch + 1);
-    const int per = (whole + ranges - 1) / ranges, mine = (int)blockIdx.x * ranges * per, end = mine + ranges * per;
+    int per = (total + p.grid - 1) / p.grid, ranges = 1;
+    if (per > p.stretch) {
+      ranges = (per - 1) / p.stretch + 1;
+      per = (per - 1) / ranges + 1;
+    }
+    const int mine = (int)blockIdx.x * ranges * per, end = mine + ranges * per;
     if (blockIdx.x == 0 || (mine >= at && mine < at + own)) {
       for (int v = v0; v < v1; ++v) {
         const int n = run == 1 ? last : pair_tiles(p, v, &len, &start), places = n > 0 ? n + p.start : 0;
@@ -709,7 +712,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     }
     // A wait that fails only makes this warp skip its later waits: every warp walks all tiles, so the
     // groups' named barriers always meet and the kernel ends (its results are NaN, and the status says so).
-    bool ok = true;
+    bool ok = !idle;
     uint32_t n_tile = 0;
     int stage = 0;  // first stage of the tile
     auto wait = [&](uint64_t* bar, uint32_t use, int code) {  // the warp is converged again behind it, and agrees
@@ -724,21 +727,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       bulk_load(sq, p.q_parts + (int64_t)v * p.q_bytes, p.q_bytes, q_full);
     };
     pdl_wait();  // the query parts are there
-    if (idle) {  // NaN for every row with a key
-      while (w.next(p, share, pairs)) {
-        const int b = w.v / p.row_tiles, row0 = (w.v - b * p.row_tiles) * p.rows_tile;
-        const int nrow = min(p.rows_tile, p.rows - row0);
-        if (w.range < 0) {
-          T* out = static_cast<T*>(p.a.out) + ((int64_t)b * p.rows + row0) * width;
-          for (int64_t i = tid - 64; i < (int64_t)nrow * width; i += 256) out[i] = from_f<T>(__uint_as_float(0x7FC00000u));
-        } else if (tid - 64 < nrow) {
-          p.part_lse[part_of(p, w.range, w.v, w.t0 == 0, pairs) * p.rows_tile + tid - 64] = __uint_as_float(0x7FC00000u);
-        }
-      }
-      __syncwarp();
-    }
-    bool have = !idle && w.next(p, share, pairs);
-    if (have && warp == 2) {
+    bool have = w.next(p, share, pairs);
+    if (have && warp == 2 && ok) {
       if (elect_one()) load_q(w.v);
       ++n_q;
     }
@@ -930,7 +920,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       }
       group_sync(bar_id);
       const bool whole = w.range < 0;
-      const int64_t part = part_of(p, w.range, w.v, w.t0 == 0, pairs);
+      const int64_t part = part_of(p, w.range, w.v, w.t0 == 0);
       if (quad == 0 && lane < RH) {
         const int r = r0 + lane;
         const float x = sred[r] + sred[R + r] + sred[2 * R + r] + sred[3 * R + r];
@@ -1024,14 +1014,18 @@ __global__ void __launch_bounds__(kJoinThreads<SL>) attn_tc_join_kernel(const __
   const int n = places - p.start;  // tiles, if any
   const int c0 = n > 0 ? (at + p.start) / per : 0, c1 = n > 0 ? (at + places - 1) / per : -1;
   if (n > 0 && c0 == c1) return;
-  auto row_of = [&](int c) { return part_of(p, c, v, c == c0, pairs) * p.rows_tile + r; };
+  // this row of the parts, one behind the other but for the first
+  const int step = p.part_c * p.rows_tile;
+  const int64_t row0_of = part_of(p, c0, v, false) * p.rows_tile + r;
+  const int more = p.part_c == 1 ? 0 : p.rows_tile;
+  auto row_of = [&](int i) { return row0_of + (int64_t)i * step + (i == 0 ? more : 0); };
   float4 acc[V];
   float m = -INFINITY, sum = 0.f;
 #pragma unroll
   for (int k = 0; k < V; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
   if constexpr (SL > 1) {  // all log-sums at once
     for (int i = threadIdx.x; i <= c1 - c0; i += kJoinThreads<SL>) {
-      const float x = p.part_lse[row_of(c0 + i)];
+      const float x = p.part_lse[row_of(i)];
       if (i < kMaxGrid) slse[i] = x;
       m = fmaxf(m, x);
     }
@@ -1050,8 +1044,8 @@ __global__ void __launch_bounds__(kJoinThreads<SL>) attn_tc_join_kernel(const __
     for (int i = 0; i < U; ++i) {
       const int ci = c + i * SL;
       const bool on = ci <= c1;
-      f[i] = !on ? -INFINITY : SL > 1 && ci - c0 < kMaxGrid ? slse[ci - c0] : p.part_lse[row_of(ci)];
-      const float* po = p.part_o + row_of(ci) * width;
+      f[i] = !on ? -INFINITY : SL > 1 && ci - c0 < kMaxGrid ? slse[ci - c0] : p.part_lse[row_of(ci - c0)];
+      const float* po = p.part_o + row_of(ci - c0) * width;
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         const int l = l0 + k * COLS * 4;
@@ -1391,7 +1385,7 @@ cudaError_t mla_attn_tc(int dtype, const MlaCacheAttnArgs& a, cudaStream_t s) {
   p.q_bytes = pl.boxes * pl.ns * 128;
   p.grid = pl.grid;
   p.start = (a.cache.slots + kTile - 1) / kTile * a.batch * pl.row_tiles <= pl.grid ? 0 : kStart;
-  p.ranges = (int)pl.ranges;
+  p.part_c = (int64_t)a.batch * pl.row_tiles <= pl.ranges ? 1 : 2;
   p.stretch = pl.stretch;
   p.fetch = kFetch;
   p.direct = pl.direct ? 1 : 0;
