@@ -44,12 +44,13 @@
 //
 // What bounds it.  One product reads its tile from shared memory once per run of weight parts, at 128 bytes a clock:
 // with 24 rows of width 1536 a tile of 96 KB is written once, read once (with 72 KB of query parts) for the scores and
-// three times (with 24 KB of weights each) for the context: by that count 4,980 clocks of a measured 6,260 (the counters
-// show 57 % of the shared-memory and L1 throughput over the whole kernel); the rest is scores -> weights -> context one
-// behind the other, since 72 KB of query parts leave a ring of one and a half tiles.
-// With 12 rows the count is 3,770 of 4,730, with 3 rows the memory bounds: 64 x 4,608 tokens of width 1536 (453 MB) take 92 - 96 us
-// for 3 heads (4.8 TB/s, 73 % of the measured copy), 158 for 24.  Under this load the GPU runs at its power limit.
-// Short calls are three launches and one tile's latency: 12.8 us for one sequence of 257 tokens on the GPU alone.
+// three times (with 24 KB of weights each) for the context: by that count 4,980 clocks of 6,260 measured between moves of
+// the accumulators (the counters show 56 % of the shared-memory and L1 throughput over the whole kernel, start, epilogue,
+// moves and waits included); the rest is scores -> weights -> context one behind the other, since 72 KB of query parts
+// leave a ring of one and a half tiles.  With 12 rows the count is 3,770 of 4,730.  64 x 4,608 tokens of width 1536 (453 MB)
+// take 168 us for 24 heads, and 97 - 98 for 3 (4.7 TB/s, 71 % of the measured copy; this kernel alone 92.6 at 76 %): memory,
+// through a ring of two tiles.  Under this load the GPU runs at its power limit.
+// Short calls are three launches and one tile's latency: 13.3 - 13.8 us for one sequence of 257 tokens.
 //
 // Roles of an attention CTA (10 warps): warp 0 loads, warp 1 issues the MMAs, warps 2-9 are two groups
 // of four that share the rows: scores -> weights, rescaling and the epilogue.

@@ -529,9 +529,10 @@ def absorbed_latent_decode(query, latent_cache, cache_mask, key_up_weight, value
 # Query tokens per row up to which a quantized cache is attended in the latent space.  Per cached token the
 # absorbed form costs 4 H L flops for every query token, rebuilding K and V 2 L H (Dq + Dv) once and
 # 2 H (Dq + Dv) per query token besides the traffic of K and V (and of the scores) through memory.  A layer's
-# forward in us, absorbed / rebuilt, at 16, 64, 128 and 256 query tokens: 64 sequences of 2,048, 10 heads, width 640
-# 603 / 2408, 1016 / 2624, 1672 / 2824, 2974 / 2793; 16 of 4,096, 24 heads, width 1536 901 / 3148, 2177 / 3310,
-# 3927 / 3436, 7472 / 3065.
+# forward in us, absorbed / rebuilt (through PyTorch's masked attention, as the layer does it for ragged rows on a
+# cache), bf16, at 16, 64, 128 and 256 query tokens: 64 sequences of 2,048, 10 heads, width 640 627 / 2425,
+# 1036 / 2624, 1722 / 2851, 3059 / 2791; 16 of 4,096, 24 heads, width 1536 915 / 3147, 2225 / 3308, 4000 / 3412,
+# 7638 / 3078.
 ABSORBED_QUERY_LIMIT = 64
 # The same where the attention runs on fp32 FMAs (fp32 layers, widths that are no multiples of 16), at 4, 8 and 16 query
 # tokens: fp32, 64 of 2,048, 10 heads, width 640 1903 / 4699, 3082 / 4710, 5418 / 4770; fp32, 16 of 4,096, 24 heads,
