@@ -332,7 +332,8 @@ class QuantizedMLACache(StaticMLACache):
 
     def attend(self, query_latent: torch.Tensor, *, query_start: torch.Tensor | None = None,
                scale: float = 1.0) -> torch.Tensor:
-        """Contexts ``[B,Tq,H,L]`` of queries absorbed into the latent space (``ops.mla_cache_attention``)."""
+        """Contexts ``[B,Tq,H,L]`` of queries absorbed into the latent space (``ops.mla_cache_attention``, which refuses
+        widths over 2,048: see ``ops.mla_cache_attention_form``)."""
         if _ops.use_kernels(query_latent):
             return _ops.mla_cache_attention(query_latent, self.latent_kv, self.scales, self.sequence_offset,
                                             query_start=query_start, scale=scale)
